@@ -298,6 +298,149 @@ int pyc_b200_symm_open(const unsigned char handle[64], void** ptr);
 int pyc_b200_symm_close(void* ptr);
 int pyc_b200_symm_free(void* ptr);
 
+/* ---- serving: 8-bit paged key/value cache, attention over it, token scores ------------------------------------------- *
+ * No counterpart in PyC (its IR has no cache, no ragged batch and no token scores).
+ *
+ * The cache is a pool of `num_blocks` blocks of `block_size` tokens (16, 32, 64 or 128).  For each block and key/value head it
+ * holds [block_size][head_dim] e4m3 codes for the keys and as many for the values (k_cache, v_cache:
+ * [num_blocks][kv_heads][block_size][head_dim] bytes) and one fp32 scale each (k_scale, v_scale: [num_blocks][kv_heads]); a
+ * code c stands for c * scale.  head_dim is 64 or 128.  Row r of the block table lists request r's blocks in the order of
+ * its tokens; the SLOT of a token is block * block_size + position within the block.  All counts, tables and free lists are
+ * device memory: a step can be captured in a CUDA graph and replayed with other lengths.
+ * None of these calls synchronises or allocates device memory.  They return 0, or -1 with a message in pyc_b200_last_error(). */
+
+/* Block tables and slot maps of one step, from the requests' lengths, in one launch.  Request r holds context_lens[r] tokens
+ * and brings new_lens[r] more (0 is allowed).  The blocks that it lacks are taken from the end of the free list in the order
+ * of the requests and entered in its table row.  All or nothing: when result[0] is one of the errors 1 | 2 | 4 | 8, no block
+ * is handed out, query_start is all 0, seq_lens = context_lens, every slot is -1, and nothing else changes.
+ *   result[0]  0, or a sum of  1 a negative length   2 a request longer than max_blocks * block_size   4 more than
+ *              max_tokens new tokens   8 too few free blocks   16 a block id outside the pool in the table or the free list
+ *              (the tokens that fall into such a block get slot -1; the rest of the step is valid)
+ *   result[1]  tokens of the step    result[2]  blocks taken    result[3]  blocks missing (error 8)
+ * Entries of slot_map and token_request from result[1] up to max_tokens are set to -1, those of positions to 0: a captured
+ * step of max_tokens rows skips them.  free_count_out may be NULL (or free_count): the count is then updated in place.  With
+ * another address for it, calling again with the same lengths plans the same step again. */
+typedef struct {
+    int requests;                  /* 1 .. 16384 */
+    int block_size, num_blocks;
+    int max_blocks;                /* entries in a row of block_table */
+    int max_tokens;                /* entries of slot_map, positions and token_request */
+    const int* context_lens;       /* [requests] */
+    const int* new_lens;           /* [requests] */
+    const int* free_blocks;        /* [num_blocks], the first *free_count of them unused block ids */
+    int* free_count;
+    int* free_count_out;           /* may be NULL */
+    int* block_table;              /* [requests][max_blocks]; entries behind a request's last block are not touched */
+    int* query_start;              /* [requests + 1]: first new token of each request */
+    int* seq_lens;                 /* [requests]: context_lens + new_lens */
+    long long* slot_map;           /* [max_tokens] */
+    int* positions;                /* [max_tokens] */
+    int* token_request;            /* [max_tokens] */
+    int* result;                   /* [4] */
+} pyc_b200_kv_plan_args;
+int pyc_b200_kv_plan(const pyc_b200_kv_plan_args* args, void* stream);
+
+/* Give the blocks of the requests with finished[r] != 0 back to the end of the free list, clear their table entries to -1 and
+ * set their context_lens to 0.  The other requests are not touched. */
+int pyc_b200_kv_release(int requests, int block_size, int num_blocks, int max_blocks, const int* finished, int* context_lens,
+                        int* block_table, int* free_blocks, int* free_count, void* stream);
+
+/* Quantise new keys and values into the cache.  k, v: [tokens][kv_heads][head_dim] bf16 or f16, rows k_stride / v_stride
+ * elements apart (0: contiguous; a multiple of 8; 16-byte aligned), so that they can be read in place from a wider
+ * projection.  Token t goes to slot_map[t]; a slot outside the pool (-1 for padding) is skipped.  Tokens with consecutive
+ * slots in one block form a run; a block may belong to ONE run of a call, and tokens earlier in that block than the run are
+ * those that it keeps (slots behind the run are not touched).
+ * The scale of a block and head is a power of two, 2^-32 .. 2^64: the smallest that brings the largest finite |x| of the run
+ * to 448 or less; a run that does not start its block takes the larger of that and the block's present scale, and when the
+ * scale grows the codes that the block keeps are rounded again to the new one (exact, but for codes that leave the normal
+ * range).  Values round to nearest even; infinities become the block's largest value, NaN stays NaN. */
+typedef struct {
+    pyc_dtype dtype;
+    int tokens, kv_heads, head_dim, block_size, num_blocks;
+    const void* k;
+    const void* v;
+    size_t k_stride, v_stride;
+    const long long* slot_map;     /* [tokens] */
+    void* k_cache;
+    void* v_cache;
+    float* k_scale;
+    float* v_scale;
+} pyc_b200_kv_write_args;
+int pyc_b200_kv_write(const pyc_b200_kv_write_args* args, void* stream);
+
+/* Attention over the cache, for any mixture of single new tokens, several tokens and long chunks:
+ *   out[t][h] = softmax(scale * q[t][h] . K) V  over the keys that token t sees,   lse[t][h] = log of the softmax's sum
+ * Request r's queries are rows query_start[r] .. query_start[r+1] - 1 of q (query_start non-decreasing, from 0); it has
+ * seq_lens[r] keys, the new ones included (written before).  Query head h reads key head h / (heads / kv_heads).  With causal != 0 query i of
+ * n sees keys 0 .. seq_lens[r] - n + i, else all.  A row that sees no key gives out = 0 and lse = -inf.  Keys of a block id
+ * outside the pool are masked.  Values behind a request's end and keys that a row does not see have no influence, NaN
+ * included.  Rows of out and lse from query_start[requests] on are not touched.  seq_lens beyond max_blocks * block_size
+ * count as that; scales outside 2^-40 .. 2^72 count as the nearer of the two.
+ * q, out: bf16 or f16, rows q_stride / out_stride elements apart (0: contiguous; a multiple of 8; 16-byte aligned), heads
+ * contiguous.  max_query is an upper bound of the queries of a request (a larger request's surplus rows are left undone),
+ * and any number of rows may stand behind the last request.  workspace: pyc_b200_paged_attention_workspace_bytes(...) bytes,
+ * 256-byte aligned, zeroed once before its first use; calls that may run at the same time need a workspace each (the
+ * calls of one stream can share one, captured graphs that never overlap too). */
+typedef struct {
+    pyc_dtype dtype;
+    int requests, max_query;       /* requests: 1 .. 16384 */
+    int heads, kv_heads, head_dim; /* heads a multiple of kv_heads */
+    int block_size, num_blocks, max_blocks;
+    const void* q;
+    const void* k_cache;
+    const void* v_cache;
+    const float* k_scale;
+    const float* v_scale;
+    const int* block_table;        /* [requests][max_blocks] */
+    const int* query_start;        /* [requests + 1] */
+    const int* seq_lens;           /* [requests] */
+    void* out;
+    float* lse;                    /* [rows][heads], may be NULL */
+    size_t q_stride, out_stride;
+    float scale;
+    int causal;
+} pyc_b200_paged_attention_args;
+size_t pyc_b200_paged_attention_workspace_bytes(int requests, int max_query, int heads, int kv_heads, int head_dim);
+int pyc_b200_paged_attention(const pyc_b200_paged_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Scores of given tokens from logits [rows][vocab] (F32, BF16 or F16; rows row_stride elements apart, 0: vocab), in one pass:
+ *   lse = log sum_j e^{x_j},  logprob = x_token - lse,  entropy = -sum_j p_j log p_j  (p = softmax, 0 log 0 = 0),
+ * and the top_k (0 .. 32, at most vocab) largest logits' indices and log probabilities, largest first, equal values by the
+ * lower index.  tokens[row] outside 0 .. vocab - 1 (-1 for "no token") gives logprob 0.  A row with nothing but -inf gives
+ * lse = -inf, entropy 0 and log probabilities -inf (top ids 0 .. top_k - 1); a row with NaN or +inf gives NaN and top ids
+ * -1.  entropy, lse, and with top_k 0 top_ids and top_logprobs, may be NULL. */
+typedef struct {
+    pyc_dtype dtype;
+    size_t rows, vocab, row_stride;
+    const void* logits;
+    const int* tokens;             /* [rows] */
+    float* logprob;                /* [rows] */
+    float* entropy;                /* [rows] */
+    float* lse;                    /* [rows] */
+    int top_k;
+    int* top_ids;                  /* [rows][top_k] */
+    float* top_logprobs;           /* [rows][top_k] */
+} pyc_b200_token_logprobs_args;
+int pyc_b200_token_logprobs(const pyc_b200_token_logprobs_args* args, void* stream);
+
+/* Gradient of sum_rows (grad_logprob * logprob + grad_entropy * entropy) with respect to the logits, from the forward
+ * call's lse and entropy:  d_j = grad_logprob (1[j = token] - p_j) - grad_entropy p_j (log p_j + entropy),  p_j = e^{x_j - lse}.
+ * A token outside the vocabulary contributes no logprob term.  A row of nothing but -inf (lse = -inf) gives zeros.
+ * grad_logprob or grad_entropy may be NULL (zero).  grad_logits has the logits' type and may be the logits themselves
+ * (same stride). */
+typedef struct {
+    pyc_dtype dtype;
+    size_t rows, vocab, row_stride, grad_stride;
+    const void* logits;
+    const int* tokens;
+    const float* lse;
+    const float* entropy;
+    const float* grad_logprob;
+    const float* grad_entropy;
+    void* grad_logits;
+} pyc_b200_token_logprobs_grad_args;
+int pyc_b200_token_logprobs_backward(const pyc_b200_token_logprobs_grad_args* args, void* stream);
+
 /* Time every registered tile configuration for (dtype, M, N, K) with CUDA
  * events, feed the measured milliseconds to PyC's registry
  * (pyc_kernel_benchmark_update_symbol) when it is linked, remember the winner

@@ -90,6 +90,35 @@ class FfnArgs(C.Structure):
                 ("w2", C.c_void_p), ("w2_scale", C.c_void_p), ("b2", C.c_void_p), ("out", C.c_void_p)]
 
 
+class KvPlanArgs(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("requests", "block_size", "num_blocks", "max_blocks", "max_tokens")] + \
+               [(n, C.c_void_p) for n in ("context_lens", "new_lens", "free_blocks", "free_count", "free_count_out", "block_table", "query_start",
+                                          "seq_lens", "slot_map", "positions", "token_request", "result")]
+
+
+class KvWriteArgs(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "tokens", "kv_heads", "head_dim", "block_size", "num_blocks")] + \
+               [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_size_t), ("v_stride", C.c_size_t)] + \
+               [(n, C.c_void_p) for n in ("slot_map", "k_cache", "v_cache", "k_scale", "v_scale")]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "requests", "max_query", "heads", "kv_heads", "head_dim", "block_size", "num_blocks", "max_blocks")] + \
+               [(n, C.c_void_p) for n in ("q", "k_cache", "v_cache", "k_scale", "v_scale", "block_table", "query_start", "seq_lens", "out", "lse")] + \
+               [("q_stride", C.c_size_t), ("out_stride", C.c_size_t), ("scale", C.c_float), ("causal", C.c_int)]
+
+
+class TokenLogprobsArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("rows", C.c_size_t), ("vocab", C.c_size_t), ("row_stride", C.c_size_t), ("logits", C.c_void_p),
+                ("tokens", C.c_void_p), ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("lse", C.c_void_p), ("top_k", C.c_int),
+                ("top_ids", C.c_void_p), ("top_logprobs", C.c_void_p)]
+
+
+class TokenLogprobsGradArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("rows", C.c_size_t), ("vocab", C.c_size_t), ("row_stride", C.c_size_t), ("grad_stride", C.c_size_t)] + \
+               [(n, C.c_void_p) for n in ("logits", "tokens", "lse", "entropy", "grad_logprob", "grad_entropy", "grad_logits")]
+
+
 class RuntimeInfo(C.Structure):
     _fields_ = [("arena_bytes", C.c_size_t), ("plan_peak_bytes", C.c_size_t), ("plan_total_bytes", C.c_size_t),
                 ("graphs_cached", C.c_size_t), ("graph_replays", C.c_size_t), ("kernels_per_graph", C.c_size_t),

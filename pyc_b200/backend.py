@@ -22,6 +22,8 @@ EXPORTS = [
     "pyc_b200_gemm", "pyc_b200_gemm_static", "pyc_b200_gemm_static_status", "pyc_b200_add", "pyc_b200_bias_act", "pyc_b200_layernorm", "pyc_b200_softmax",
     "pyc_b200_reduce_sum", "pyc_b200_quantize_rows", "pyc_b200_layernorm_quantize", "pyc_b200_gemm_fp8",
     "pyc_b200_ffn_workspace_bytes", "pyc_b200_ffn_block", "pyc_b200_ffn_block_tp", "pyc_b200_ffn_phase_events", "pyc_b200_ffn_block_scatter", "pyc_b200_tp_reduce_broadcast", "pyc_b200_tp_allreduce_multimem", "pyc_b200_ffn_block_switch_reduce",
+    "pyc_b200_kv_plan", "pyc_b200_kv_release", "pyc_b200_kv_write", "pyc_b200_paged_attention_workspace_bytes", "pyc_b200_paged_attention",
+    "pyc_b200_token_logprobs", "pyc_b200_token_logprobs_backward",
     "pyc_b200_symm_alloc", "pyc_b200_symm_open", "pyc_b200_symm_close", "pyc_b200_symm_free", "pyc_b200_attention", "pyc_b200_conv2d", "pyc_b200_autotune_gemm", "pyc_b200_autotune_db_load", "pyc_b200_last_plan", "pyc_b200_plan_arena",
     "pyc_b200_get_runtime_info", "pyc_b200_set_stream", "pyc_b200_device_status", "pyc_b200_selftest_wait_timeout", "pyc_b200_last_error",
     "pyc_b200_shutdown",
@@ -79,6 +81,14 @@ def load():
     L.pyc_b200_symm_open.argtypes = [C.c_char_p, C.POINTER(vp)]
     L.pyc_b200_symm_close.argtypes = [vp]
     L.pyc_b200_symm_free.argtypes = [vp]
+    L.pyc_b200_kv_plan.argtypes = [C.POINTER(abi.KvPlanArgs), vp]
+    L.pyc_b200_kv_release.argtypes = [i, i, i, i, vp, vp, vp, vp, vp, vp]
+    L.pyc_b200_kv_write.argtypes = [C.POINTER(abi.KvWriteArgs), vp]
+    L.pyc_b200_paged_attention_workspace_bytes.argtypes = [i, i, i, i, i]
+    L.pyc_b200_paged_attention_workspace_bytes.restype = sz
+    L.pyc_b200_paged_attention.argtypes = [C.POINTER(abi.PagedAttentionArgs), vp, sz, vp]
+    L.pyc_b200_token_logprobs.argtypes = [C.POINTER(abi.TokenLogprobsArgs), vp]
+    L.pyc_b200_token_logprobs_backward.argtypes = [C.POINTER(abi.TokenLogprobsGradArgs), vp]
     L.pyc_b200_attention.argtypes = [i, i, i, i, vp, vp, vp, vp, f, i, vp]
     L.pyc_b200_conv2d.argtypes = [i] * 12 + [vp, vp, vp, i, vp, vp]
     L.pyc_b200_autotune_gemm.argtypes = [i, i, i, i, i, C.c_char_p, sz, C.POINTER(C.c_double)]
@@ -319,6 +329,56 @@ def symm_free(ptr):
 
 def attention(dtype, batch_heads, seq, d, q, k, v, out, scale, causal, stream=0):
     _check(load().pyc_b200_attention(dtype, batch_heads, seq, d, q, k, v, out, scale, int(causal), stream), "pyc_b200_attention")
+
+
+def kv_plan(requests, block_size, max_blocks, max_tokens, num_blocks, context_lens, new_lens, free_blocks, free_count, block_table,
+            query_start, seq_lens, slot_map, positions, token_request, result, free_count_out=None, stream=0):
+    """Block tables and slot maps of a step from the requests' lengths (all pointers: device, see include/pyc_b200.h)."""
+    a = abi.KvPlanArgs(requests, block_size, num_blocks, max_blocks, max_tokens, context_lens, new_lens, free_blocks, free_count,
+                       free_count_out, block_table, query_start, seq_lens, slot_map, positions, token_request, result)
+    _check(load().pyc_b200_kv_plan(C.byref(a), stream), "pyc_b200_kv_plan")
+
+
+def kv_release(requests, block_size, max_blocks, num_blocks, finished, context_lens, block_table, free_blocks, free_count, stream=0):
+    """Give the blocks of the requests with finished[r] != 0 back to the free list."""
+    _check(load().pyc_b200_kv_release(requests, block_size, num_blocks, max_blocks, finished, context_lens, block_table, free_blocks,
+                                      free_count, stream), "pyc_b200_kv_release")
+
+
+def kv_write(dtype, tokens, kv_heads, head_dim, block_size, num_blocks, k, v, slot_map, k_cache, v_cache, k_scale, v_scale,
+             k_stride=0, v_stride=0, stream=0):
+    """Quantise keys and values (e4m3, one power-of-two scale per block and head) into their slots of the paged cache."""
+    a = abi.KvWriteArgs(dtype, tokens, kv_heads, head_dim, block_size, num_blocks, k, v, k_stride, v_stride, slot_map, k_cache, v_cache,
+                        k_scale, v_scale)
+    _check(load().pyc_b200_kv_write(C.byref(a), stream), "pyc_b200_kv_write")
+
+
+def paged_attention_workspace_bytes(requests, max_query, heads, kv_heads, head_dim):
+    return int(load().pyc_b200_paged_attention_workspace_bytes(requests, max_query, heads, kv_heads, head_dim))
+
+
+def paged_attention(dtype, requests, max_query, heads, kv_heads, head_dim, block_size, num_blocks, max_blocks, q, k_cache, v_cache, k_scale,
+                    v_scale, block_table, query_start, seq_lens, out, scale, causal, workspace, workspace_bytes, lse=None, q_stride=0,
+                    out_stride=0, stream=0):
+    """Attention of a ragged batch of queries over the 8-bit paged cache."""
+    a = abi.PagedAttentionArgs(dtype, requests, max_query, heads, kv_heads, head_dim, block_size, num_blocks, max_blocks, q, k_cache, v_cache,
+                               k_scale, v_scale, block_table, query_start, seq_lens, out, lse, q_stride, out_stride, scale, int(causal))
+    _check(load().pyc_b200_paged_attention(C.byref(a), workspace, workspace_bytes, stream), "pyc_b200_paged_attention")
+
+
+def token_logprobs(dtype, rows, vocab, logits, tokens, logprob, entropy=None, lse=None, top_k=0, top_ids=None, top_logprobs=None,
+                   row_stride=0, stream=0):
+    """Log probability of each row's token, entropy, log-sum-exp and the top_k alternatives of logits [rows, vocab]."""
+    a = abi.TokenLogprobsArgs(dtype, rows, vocab, row_stride, logits, tokens, logprob, entropy, lse, top_k, top_ids, top_logprobs)
+    _check(load().pyc_b200_token_logprobs(C.byref(a), stream), "pyc_b200_token_logprobs")
+
+
+def token_logprobs_backward(dtype, rows, vocab, logits, tokens, lse, entropy, grad_logprob, grad_entropy, grad_logits, row_stride=0,
+                            grad_stride=0, stream=0):
+    """Gradient of token_logprobs' logprob and entropy with respect to the logits."""
+    a = abi.TokenLogprobsGradArgs(dtype, rows, vocab, row_stride, grad_stride, logits, tokens, lse, entropy, grad_logprob, grad_entropy,
+                                  grad_logits)
+    _check(load().pyc_b200_token_logprobs_backward(C.byref(a), stream), "pyc_b200_token_logprobs_backward")
 
 
 def conv2d(dtype, N, H, W, Cin, K, R, S, pad, stride, x, w, bias, relu, out, stream=0):
