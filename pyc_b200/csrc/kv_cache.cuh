@@ -20,6 +20,10 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
     asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(h) : "r"(two));
     return h;
 }
+// Four codes: the two low ones and the two high ones.
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t four, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
+}
 __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t two) {
     const uint32_t h = e4m3x2_to_f16x2(two);
     return __half22float2(*reinterpret_cast<const __half2*>(&h));

@@ -2,10 +2,10 @@
 // PyC has no counterpart; the dense kernels are in attention.cu.
 //
 // This file: few query rows per key head (single new tokens, a few of them, grouped heads), which is bound by reading the
-// cache.  A CTA walks the items of its stretch (paged_attention.cuh).  Each of its eight warps takes 16 keys of a unit
-// of 128 and runs on its own: its own ring of TMA loads (keys and values of 16 tokens, one copy each, into 128-byte
-// swizzled shared memory), its own running maximum and sums in registers, no barrier with the other warps before the
-// item's end.  A 16-token group never crosses a block (block sizes are multiples of 16).
+// cache.  A CTA walks the items of its stretch (paged_attention.cuh).  Each of its warps takes 32 keys of every unit
+// and runs on its own: its own ring of TMA loads (keys and values, one copy each or two where a block is 16 tokens, into
+// 128-byte swizzled shared memory), its own running maximum and sums in registers, no barrier with the other warps before
+// the item's end.
 //
 // Products: mma m16n8k16, f16 x f16 -> f32, 16 rows of the tile at a time.  The codes become f16 exactly, one conversion per
 // two codes, straight into operand registers:
@@ -23,6 +23,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <climits>
 
 #include "internal.h"
@@ -32,24 +33,28 @@
 namespace b200 {
 namespace {
 
-constexpr int NW = 8;                        // warps per CTA
-constexpr int THREADS = NW * 32;
-constexpr int UNIT = NW * 16;                // keys per unit
+constexpr int GROUP = 32;                    // keys that a warp takes at a time
 
+// MT: 16-row tiles per item.
 template <int D, int MT>
-struct ShortSmem {
-    static constexpr int TILE = 16 * D;                                    // bytes of 16 keys (or values)
-    static constexpr int STAGES = (MT == 1 ? 24576 : 49152) / (NW / 4 * 2 * TILE);   // MT 1: 96 KB of ring, two CTAs per SM; MT 2: 192 KB, one
-    static constexpr int RING = NW * STAGES * 2 * TILE;
-    static constexpr int Q_OFF = RING;
+struct ShortCfg {
+    static constexpr int NW = MT == 1 ? 4 : 8;                             // warps per CTA
+    static constexpr int PER_SM = MT == 1 ? 3 : 1;                         // resident CTAs
+    static constexpr int THREADS = NW * 32;
+    static constexpr int UNIT = NW * GROUP;                                // keys per unit
+    static constexpr int TILE = GROUP * D;                                 // bytes of a group's keys (or values)
+    static constexpr int RING_BYTES = (MT == 1 ? 64 : 192) * 1024;
+    static constexpr int STAGES = RING_BYTES / (NW * 2 * TILE);
+    static constexpr int Q_OFF = RING_BYTES;
     static constexpr int Q_BYTES = MT * 16 * D * 2;
     static constexpr int ROW_OFF = Q_OFF + Q_BYTES;                        // float [MT * 16] row scales
     static constexpr int ML_OFF = ROW_OFF + MT * 16 * 4;                   // float [NW][MT * 16][2]
-    static constexpr int INFO_OFF = ML_OFF + NW * MT * 16 * 8;             // float4 [NW][STAGES]
-    static constexpr int BAR_OFF = INFO_OFF + NW * STAGES * 16;            // mbarriers [NW][STAGES]
+    static constexpr int INFO_OFF = ML_OFF + NW * MT * 16 * 8;             // float4 [NW][STAGES][2]
+    static constexpr int BAR_OFF = INFO_OFF + NW * STAGES * 32;            // mbarriers [NW][STAGES]
     static constexpr int MISC_OFF = BAR_OFF + NW * STAGES * 8;             // long long [NW], int flag
     static constexpr int BYTES = MISC_OFF + NW * 8 + 16 + 1024;            // + alignment
-    static_assert(NW * MT * 16 * D * 4 <= RING, "the ring holds the warps' sums at an item's end");
+    static_assert(NW * MT * 16 * D * 4 <= RING_BYTES, "the ring holds the warps' sums at an item's end");
+    static_assert(STAGES >= 2 && STAGES <= 32 && (BYTES + 1024) * PER_SM <= 228 * 1024, "shared memory of an SM");
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -77,18 +82,18 @@ template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-// MT: 16-row tiles per item (1 or 2).
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(THREADS, MT == 1 ? 2 : 1)
-paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PagedParams p) {
-    using SM = ShortSmem<D, MT>;
+__global__ void __launch_bounds__(ShortCfg<D, MT>::THREADS, ShortCfg<D, MT>::PER_SM)
+paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PagedParams p, int halves) {
+    using SM = ShortCfg<D, MT>;
+    constexpr int NW = SM::NW, THREADS = SM::THREADS, UNIT = SM::UNIT;
     constexpr int TILE = MT * 16, S = SM::STAGES, KC = D / 64, NT = D / 8;   // KC: 16-byte chunks of a key per thread; NT: column tiles
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c4 = lane & 3;
     float* row_scale = reinterpret_cast<float*>(smem + SM::ROW_OFF);
     float* warp_ml = reinterpret_cast<float*>(smem + SM::ML_OFF);
-    float4* info = reinterpret_cast<float4*>(smem + SM::INFO_OFF) + w * S;
+    float4* info = reinterpret_cast<float4*>(smem + SM::INFO_OFF) + w * S * 2;
     const uint32_t bars = smem_u32(smem + SM::BAR_OFF) + w * S * 8;
     const uint32_t ring = smem_u32(smem) + w * S * 2 * SM::TILE;
     const uint32_t q_frags = smem_u32(smem + SM::Q_OFF) + lane * 16;
@@ -96,7 +101,7 @@ paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     int* flag = reinterpret_cast<int*>(scratch + NW);
 
     if (lane == 0) {
-        for (int i = 0; i < S; ++i) mbar_init(bars + 8 * i, 1);
+        for (int i = 0; i < S; ++i) mbar_init(bars + 8 * i, halves);
         fence_barrier_init();
         fence_proxy_async();
         if (w == 0) { prefetch_tmap(&tmK); prefetch_tmap(&tmV); }
@@ -107,6 +112,14 @@ paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     if (!busy) return;
     uint32_t phases = 0;                     // parity of each stage's next completion
     bool ok = true;
+    // this thread's places in a stage: keys g (+ 8, 16, 24) and values 2c, 2c + 1 (+ 8, ...).  8 lines on the swizzle repeats: that
+    // is 8 keys for D = 128 and 16 for D = 64, where 8 keys on the chunk's bit 2 (64 bytes) is the other one
+    constexpr int ODD = D == 64 ? 64 : 0;
+    uint32_t k_at[KC][2], v_at[2][2];
+#pragma unroll
+    for (int i = 0; i < KC; ++i) { k_at[i][0] = swizzled(g * D + c4 * (D / 4) + i * 16); k_at[i][1] = k_at[i][0] ^ ODD; }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) { v_at[i][0] = swizzled((2 * c4 + i) * D + g * NT); v_at[i][1] = v_at[i][0] ^ ODD; }
 
     for (long long u = c.lo; u < c.hi;) {
         const int j0 = static_cast<int>(u - c.item), j1 = static_cast<int>(min(static_cast<long long>(c.units), c.hi - c.item));
@@ -114,35 +127,40 @@ paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         const int kend = paged_tile_end<TILE>(p, c.q, c.t);
         const int* table = p.table + static_cast<size_t>(c.r) * p.max_blocks;
 
-        // ---- the ring: lane l holds block id and scales of unit base + l's group; that lane issues its copies
+        // ---- the ring.  A group lies in one block (halves = 1, block sizes from 32) or in two of 16 tokens (halves = 2).  Lane
+        // (j - base) * halves + i holds id and scales of half i of unit j's group, and issues its copies.
         int base = j0, id = -1;
-        float ks = 0.0f, vs = 1.0f;
+        float4 about = make_float4(0.0f, 0.0f, 1.0f, 0.0f);                  // key scale (0: masked), log2 of the value scale, 1 / it
         auto fetch = [&](int j) {
             base = j;
-            const long long key = (static_cast<long long>(j) + lane) * UNIT + w * 16;
+            const int mine = j + (halves == 2 ? lane >> 1 : lane);
+            const long long key = static_cast<long long>(mine) * UNIT + w * GROUP + (halves == 2 ? (lane & 1) * 16 : 0);
             id = -1;
-            if (j + lane < j1 && key < kend) {
+            if (mine < j1 && key < kend) {
                 id = __ldg(table + (key >> p.shift));
                 if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.num_blocks)) id = -1;
             }
+            about.x = 0.0f;
             if (id >= 0) {
                 const size_t at = static_cast<size_t>(id) * p.kv_heads + c.h;
-                ks = paged_clamp_scale(__ldg(p.k_scale + at));
-                vs = paged_clamp_scale(__ldg(p.v_scale + at));
+                const float vs = paged_clamp_scale(__ldg(p.v_scale + at));
+                about = make_float4(paged_clamp_scale(__ldg(p.k_scale + at)), log2f(vs), 1.0f / vs, 0.0f);
             }
         };
         auto issue = [&](int j, int st) {    // warp-uniform
             if (j >= j1 || !ok) return;
-            if (j - base >= 32) fetch(j);
-            if (lane == j - base) {
-                info[st] = make_float4(id >= 0 ? ks : 0.0f, log2f(vs), 1.0f / vs, 0.0f);
+            if ((j - base) * halves >= 32) fetch(j);
+            const int i = lane - (j - base) * halves;
+            if (i >= 0 && i < halves) {
+                info[st * 2 + i] = about;
+                if (halves == 1) info[st * 2 + 1] = about;
                 if (id >= 0) {
-                    const uint32_t dst = ring + st * 2 * SM::TILE;
-                    const int y = ((j * UNIT + w * 16) & (p.block_size - 1)) * D / 128, z = id * p.kv_heads + c.h;
-                    mbar_arrive_expect_tx(bars + 8 * st, 2 * SM::TILE);
+                    const uint32_t bytes = SM::TILE / halves, dst = ring + st * 2 * SM::TILE + i * (SM::TILE / 2);
+                    const int y = ((j * UNIT + w * GROUP + i * 16) & (p.block_size - 1)) * D / 128, z = id * p.kv_heads + c.h;
+                    mbar_arrive_expect_tx(bars + 8 * st, 2 * bytes);
                     tma_load_3d(dst, &tmK, bars + 8 * st, 0, y, z);
                     tma_load_3d(dst + SM::TILE, &tmV, bars + 8 * st, 0, y, z);
-                }
+                } else mbar_arrive(bars + 8 * st);
             }
         };
         fetch(j0);
@@ -151,8 +169,8 @@ paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 
         // ---- queries to f16 operand order: 16 threads per row, D / 16 values each
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const int row = mt * 16 + (threadIdx.x >> 4), x = threadIdx.x & 15;
+        for (int part = 0; part < TILE * 16 / THREADS; ++part) {
+            const int row = part * (THREADS / 16) + (threadIdx.x >> 4), mt = row >> 4, x = threadIdx.x & 15;
             constexpr int NV = D / 16;
             float v[NV];
             float amax = 0.0f;
@@ -221,80 +239,65 @@ paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 #pragma unroll 1
         for (int j = j0; j < j1; ++j) {
             __syncwarp();
-            const float4 in = info[st];
-            if (in.x > 0.0f && ok) {
+            const float4 in0 = info[st * 2], in1 = info[st * 2 + 1];
+            if (ok) {
                 ok = __all_sync(0xffffffffu, mbar_wait(bars + 8 * st, (phases >> st) & 1, p.status, 0x61));
                 phases ^= 1u << st;
             }
-            if (in.x > 0.0f && ok) {
-                const uint32_t kt = ring + st * 2 * SM::TILE, vt = kt + SM::TILE;
-                const int key0 = j * UNIT + w * 16;
-                float s[MT][2][4];
+            if (ok && (in0.x > 0.0f || in1.x > 0.0f)) {
+                const uint32_t kt = ring + st * 2 * SM::TILE;
+                const int key0 = j * UNIT + w * GROUP;
+                float s[MT][4][4];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
+                    for (int t = 0; t < 4; ++t)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[mt][t][i] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < KC; ++i) {
-                    const uint4 k0 = lds128(kt + swizzled(g * D + c4 * (D / 4) + i * 16)), k1 = lds128(kt + swizzled((g + 8) * D + c4 * (D / 4) + i * 16));
-                    const uint32_t a0[4] = {k0.x, k0.y, k0.z, k0.w}, a1[4] = {k1.x, k1.y, k1.z, k1.w};
+                    uint4 kk[4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) kk[t] = lds128(kt + k_at[i][t & 1] + t * 8 * D);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        const uint32_t b00 = e4m3x2_to_f16x2(a0[x] & 0xffffu), b01 = e4m3x2_to_f16x2(a0[x] >> 16);
-                        const uint32_t b10 = e4m3x2_to_f16x2(a1[x] & 0xffffu), b11 = e4m3x2_to_f16x2(a1[x] >> 16);
+                        uint32_t b[4][2];
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) e4m3x4_to_f16x4(x == 0 ? kk[t].x : x == 1 ? kk[t].y : x == 2 ? kk[t].z : kk[t].w, b[t][0], b[t][1]);
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
                             const uint4 qa = lds128(q_frags + (mt * (D / 16) + i * 4 + x) * 512);
                             const uint32_t a[4] = {qa.x, qa.y, qa.z, qa.w};
-                            mma_f16(s[mt][0], a, b00, b01);
-                            mma_f16(s[mt][1], a, b10, b11);
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) mma_f16(s[mt][t], a, b[t][0], b[t][1]);
                         }
                     }
                 }
-                // values: rows 2c, 2c + 1, 2c + 8, 2c + 9 of the group, D / 8 codes each
-                uint32_t v[4][NT / 4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t a = vt + swizzled((2 * c4 + (i & 1) + (i >> 1) * 8) * D + g * NT);
-                    if constexpr (NT == 16) { const uint4 x = lds128(a); v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w; }
-                    else { const uint2 x = lds64(a); v[i][0] = x.x; v[i][1] = x.y; }
-                }
-                const bool cut = key0 + 16 > all_see;                        // some row does not see some key of the group
-                bool own_nan = false;
-                if (cut) {
-                    uint32_t nans = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const bool past = key0 + 2 * c4 + (i & 1) + (i >> 1) * 8 >= kend;
-#pragma unroll
-                        for (int x = 0; x < NT / 4; ++x) {
-                            if (past) v[i][x] = 0;                           // behind the last key of the tile: whatever is there
-                            const uint32_t z = nan_codes(v[i][x]);
-                            nans |= z;
-                            v[i][x] &= ~((z >> 7) * 0xffu);                  // 0 * NaN would reach the rows that do not see it
-                        }
-                    }
-                    own_nan = __any_sync(0xffffffffu, nans != 0);
-                }
-                uint32_t pa[MT][4];
+                const bool cut = key0 + GROUP > all_see || in0.x == 0.0f || in1.x == 0.0f;      // some row does not see some key of the group
+                uint32_t pa[MT][2][4];
                 bool moved = false;
                 float alpha[MT][2];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float f = qs[mt][i] * in.x;
-                        float x[4] = {fmaf(s[mt][0][2 * i], f, in.y), fmaf(s[mt][0][2 * i + 1], f, in.y), fmaf(s[mt][1][2 * i], f, in.y), fmaf(s[mt][1][2 * i + 1], f, in.y)};
-                        if (cut) {
-                            const int k = key0 + 2 * c4;
-                            if (k >= lim[mt][i]) x[0] = -INFINITY;
-                            if (k + 1 >= lim[mt][i]) x[1] = -INFINITY;
-                            if (k + 8 >= lim[mt][i]) x[2] = -INFINITY;
-                            if (k + 9 >= lim[mt][i]) x[3] = -INFINITY;
+                        const float f0 = qs[mt][i] * in0.x, f1 = qs[mt][i] * in1.x;
+                        float x[8];
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            x[2 * t] = fmaf(s[mt][t][2 * i], t < 2 ? f0 : f1, t < 2 ? in0.y : in1.y);
+                            x[2 * t + 1] = fmaf(s[mt][t][2 * i + 1], t < 2 ? f0 : f1, t < 2 ? in0.y : in1.y);
                         }
-                        float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                        if (cut) {
+                            const int left = lim[mt][i] - key0 - 2 * c4;
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) {
+                                const bool gone = (t < 2 ? in0.x : in1.x) == 0.0f;
+                                if (gone || t * 8 >= left) x[2 * t] = -INFINITY;
+                                if (gone || t * 8 + 1 >= left) x[2 * t + 1] = -INFINITY;
+                            }
+                        }
+                        float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                         const bool move = mx > m[mt][i] + 8.0f;              // also from -inf
@@ -302,11 +305,14 @@ paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                         if (move) m[mt][i] = mx;
                         moved |= move;
                         const float ref = m[mt][i] == -INFINITY ? 0.0f : m[mt][i];
-                        const float p0 = ex2_approx(x[0] - ref), p1 = ex2_approx(x[1] - ref), p2 = ex2_approx(x[2] - ref), p3 = ex2_approx(x[3] - ref);
-                        l[mt][i] = fmaf((p0 + p1) + (p2 + p3), in.z, l[mt][i] * alpha[mt][i]);
-                        const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
-                        pa[mt][i] = *reinterpret_cast<const uint32_t*>(&h0);
-                        pa[mt][2 + i] = *reinterpret_cast<const uint32_t*>(&h1);
+#pragma unroll
+                        for (int t = 0; t < 8; ++t) x[t] = ex2_approx(x[t] - ref);
+                        l[mt][i] = fmaf((x[0] + x[1]) + (x[2] + x[3]), in0.z, fmaf((x[4] + x[5]) + (x[6] + x[7]), in1.z, l[mt][i] * alpha[mt][i]));
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            const __half2 h = __floats2half2_rn(x[2 * t], x[2 * t + 1]);
+                            pa[mt][t >> 1][(t & 1) * 2 + i] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
                     }
                 }
                 if (__any_sync(0xffffffffu, moved)) {
@@ -317,35 +323,65 @@ paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 #pragma unroll
                             for (int i = 0; i < 4; ++i) o[mt][n][i] *= alpha[mt][i >> 1];
                 }
+                // values, 16 keys at a time: rows 2c, 2c + 1, 2c + 8, 2c + 9, D / 8 codes each
 #pragma unroll
-                for (int x = 0; x < NT / 4; ++x) {
-                    // bytes of two keys side by side: (key, key + 1) for columns 4x, 4x + 1 | 4x + 2, 4x + 3
-                    const uint32_t lo0 = prmt(v[0][x], v[1][x], 0x5140), lo1 = prmt(v[0][x], v[1][x], 0x7362);
-                    const uint32_t hi0 = prmt(v[2][x], v[3][x], 0x5140), hi1 = prmt(v[2][x], v[3][x], 0x7362);
-                    const uint32_t b0[4] = {e4m3x2_to_f16x2(lo0 & 0xffffu), e4m3x2_to_f16x2(lo0 >> 16), e4m3x2_to_f16x2(lo1 & 0xffffu), e4m3x2_to_f16x2(lo1 >> 16)};
-                    const uint32_t b1[4] = {e4m3x2_to_f16x2(hi0 & 0xffffu), e4m3x2_to_f16x2(hi0 >> 16), e4m3x2_to_f16x2(hi1 & 0xffffu), e4m3x2_to_f16x2(hi1 >> 16)};
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t v[4][NT / 4];
 #pragma unroll
-                    for (int y = 0; y < 4; ++y)
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t a = kt + SM::TILE + v_at[i & 1][i >> 1] + (half * 16 + (i >> 1) * 8) * D;
+                        if constexpr (NT == 16) { const uint4 x = lds128(a); v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w; }
+                        else { const uint2 x = lds64(a); v[i][0] = x.x; v[i][1] = x.y; }
+                    }
+                    bool own_nan = false;
+                    if (cut) {
+                        const bool gone = (half ? in1.x : in0.x) == 0.0f;
+                        uint32_t nans = 0;
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][4 * x + y], pa[mt], b0[y], b1[y]);
-                }
-                if (own_nan) {                                               // NaN values in a group that not every row sees whole: only to those that see them
-                    for (int k = 0; k < 16; ++k) {
-                        if (key0 + k >= kend) break;
+                        for (int i = 0; i < 4; ++i) {
+                            const bool past = gone || key0 + half * 16 + 2 * c4 + (i & 1) + (i >> 1) * 8 >= kend;
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int y = 0; y < 2; ++y) {
-                                uint32_t byte;
-                                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(vt + swizzled(k * D + (2 * c4 + y) * NT + n)));
-                                if ((byte & 127u) == 127u) {
-#pragma unroll
-                                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                                        for (int i = 0; i < 2; ++i)
-                                            if (key0 + k < lim[mt][i]) o[mt][n][2 * i + y] = __int_as_float(0x7fffffff);
-                                }
+                            for (int x = 0; x < NT / 4; ++x) {
+                                if (past) v[i][x] = 0;                       // behind the last key of the tile: whatever is there
+                                const uint32_t z = nan_codes(v[i][x]);
+                                nans |= z;
+                                v[i][x] &= ~((z >> 7) * 0xffu);              // 0 * NaN would reach the rows that do not see it
                             }
+                        }
+                        own_nan = __any_sync(0xffffffffu, nans != 0);
+                    }
+#pragma unroll
+                    for (int x = 0; x < NT / 4; ++x) {
+                        // bytes of two keys side by side: (key, key + 1) for columns 4x, 4x + 1 | 4x + 2, 4x + 3
+                        uint32_t b0[4], b1[4];
+                        e4m3x4_to_f16x4(prmt(v[0][x], v[1][x], 0x5140), b0[0], b0[1]);
+                        e4m3x4_to_f16x4(prmt(v[0][x], v[1][x], 0x7362), b0[2], b0[3]);
+                        e4m3x4_to_f16x4(prmt(v[2][x], v[3][x], 0x5140), b1[0], b1[1]);
+                        e4m3x4_to_f16x4(prmt(v[2][x], v[3][x], 0x7362), b1[2], b1[3]);
+#pragma unroll
+                        for (int y = 0; y < 4; ++y)
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][4 * x + y], pa[mt][half], b0[y], b1[y]);
+                    }
+                    if (own_nan) {                                           // NaN values in a group that not every row sees whole: only to the rows that see them
+                        for (int k = 0; k < 16; ++k) {
+                            const int key = key0 + half * 16 + k;
+                            if (key >= kend) break;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int y = 0; y < 2; ++y) {
+                                    uint32_t byte;
+                                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(kt + SM::TILE + swizzled((half * 16 + k) * D + (2 * c4 + y) * NT + n)));
+                                    if ((byte & 127u) == 127u) {
+#pragma unroll
+                                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                                            for (int i = 0; i < 2; ++i)
+                                                if (key < lim[mt][i]) o[mt][n][2 * i + y] = __int_as_float(0x7fffffff);
+                                    }
+                                }
+                        }
                     }
                 }
             }
@@ -412,15 +448,12 @@ paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     if (!ok) for (int i = 0; i < 2000; ++i) __nanosleep(1000);               // a wait has run out: let what is in flight land
 }
 
-template <int D, int MT>
-int short_ctas() { return sm_count() * (MT == 1 ? 2 : 1); }
-
 template <typename T, int D, int MT>
-int launch_short(const CUtensorMap& tmK, const CUtensorMap& tmV, const PagedParams& p, cudaStream_t s) {
-    using SM = ShortSmem<D, MT>;
+int launch_short(const CUtensorMap& tmK, const CUtensorMap& tmV, const PagedParams& p, int halves, cudaStream_t s) {
+    using SM = ShortCfg<D, MT>;
     auto kernel = paged_short_kernel<T, D, MT>;
     B200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES));
-    kernel<<<short_ctas<D, MT>(), THREADS, SM::BYTES, s>>>(tmK, tmV, p);
+    kernel<<<sm_count() * SM::PER_SM, SM::THREADS, SM::BYTES, s>>>(tmK, tmV, p, halves);
     B200_CUDA_OK(cudaGetLastError());
     count_launch();
     return 0;
@@ -428,9 +461,10 @@ int launch_short(const CUtensorMap& tmK, const CUtensorMap& tmV, const PagedPara
 
 constexpr size_t WS_COUNTERS = 4096;          // bytes: one int per CTA, at most 1024
 
-size_t partial_bytes(int head_dim, bool wide) {
-    const int tile = wide ? 32 : 16;
-    return static_cast<size_t>(sm_count()) * (wide ? 1 : 2) * 2 * tile * (head_dim + 2) * sizeof(float);
+// Two slots of [rows][D + 2] floats per CTA, for the larger of the two forms (one or two 16-row tiles).
+size_t partial_bytes(int head_dim) {
+    const int rows = std::max(ShortCfg<64, 1>::PER_SM * 16, ShortCfg<64, 2>::PER_SM * 32);
+    return static_cast<size_t>(sm_count()) * rows * 2 * (head_dim + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -442,7 +476,7 @@ extern "C" {
 
 size_t pyc_b200_paged_attention_workspace_bytes(int requests, int max_query, int heads, int kv_heads, int head_dim) {
     if (requests < 1 || max_query < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
-    return WS_COUNTERS + partial_bytes(head_dim, true);
+    return WS_COUNTERS + partial_bytes(head_dim);
 }
 
 int pyc_b200_paged_attention(const pyc_b200_paged_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -484,13 +518,14 @@ int pyc_b200_paged_attention(const pyc_b200_paged_attention_args* a, void* works
     CUtensorMap tmK, tmV;
     const uint64_t tile = static_cast<uint64_t>(a->block_size) * a->head_dim;
     const uint64_t dims[3] = {128, tile / 128, static_cast<uint64_t>(a->num_blocks) * a->kv_heads}, strides[2] = {128, tile};
-    const uint32_t box[3] = {128, static_cast<uint32_t>(16 * a->head_dim / 128), 1};
+    const int halves = a->block_size < GROUP ? 2 : 1;
+    const uint32_t box[3] = {128, static_cast<uint32_t>(GROUP / halves * a->head_dim / 128), 1};
     if (encode_tmap(&tmK, a->k_cache, 1, 3, dims, strides, box, true) != 0 || encode_tmap(&tmV, a->v_cache, 1, 3, dims, strides, box, true) != 0) return -1;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const long long most = static_cast<long long>(a->max_query) * p.group;
     p.rows_above = 0; p.rows_upto = INT_MAX;
     const bool wide = most > 16, half = a->dtype == PYC_DTYPE_F16;
-#define B200_SHORT(D, MT) (half ? launch_short<__half, D, MT>(tmK, tmV, p, s) : launch_short<__nv_bfloat16, D, MT>(tmK, tmV, p, s))
+#define B200_SHORT(D, MT) (half ? launch_short<__half, D, MT>(tmK, tmV, p, halves, s) : launch_short<__nv_bfloat16, D, MT>(tmK, tmV, p, halves, s))
     if (a->head_dim == 128) return wide ? B200_SHORT(128, 2) : B200_SHORT(128, 1);
     return wide ? B200_SHORT(64, 2) : B200_SHORT(64, 1);
 #undef B200_SHORT
