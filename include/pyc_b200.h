@@ -374,8 +374,8 @@ int pyc_b200_kv_write(const pyc_b200_kv_write_args* args, void* stream);
  * seq_lens[r] keys, the new ones included (written before).  Query head h reads key head h / (heads / kv_heads).  With causal != 0 query i of
  * n sees keys 0 .. seq_lens[r] - n + i, else all.  A row that sees no key gives out = 0 and lse = -inf.  Keys of a block id
  * outside the pool are masked.  Values behind a request's end and keys that a row does not see have no influence, NaN
- * included.  Rows of out and lse from query_start[requests] on are not touched.  seq_lens beyond max_blocks * block_size
- * count as that; scales outside 2^-40 .. 2^72 count as the nearer of the two.
+ * included.  Rows of out and lse from query_start[requests] on are not touched.  scale is positive and finite.
+ * seq_lens beyond max_blocks * block_size count as that; scales outside 2^-40 .. 2^72 count as the nearer of the two.
  * q, out: bf16 or f16, rows q_stride / out_stride elements apart (0: contiguous; a multiple of 8; 16-byte aligned), heads
  * contiguous.  max_query is an upper bound of the queries of a request (a larger request's surplus rows are left undone),
  * and any number of rows may stand behind the last request.  workspace: pyc_b200_paged_attention_workspace_bytes(...) bytes,

@@ -3,28 +3,39 @@
 //
 // This file: few query rows per key head (single new tokens, a few of them, grouped heads), which is bound by reading the
 // cache.  A CTA walks the items of its stretch (paged_attention.cuh).  Each of its warps takes 32 keys of every unit
-// and runs on its own: its own ring of TMA loads (keys and values, one copy each or two where a block is 16 tokens, into
+// and runs on its own: its own ring of TMA copies (keys and values, one copy each or two where a block is 16 tokens, into
 // 128-byte swizzled shared memory), its own running maximum and sums in registers, no barrier with the other warps before
-// the item's end.
+// the item's end.  At an item's end the next item's first copies are asked for before the warps' sums are joined, and split
+// items are announced at the end of the stretch: an item's end costs 5 to 9 us of waiting for ids, scales, queries, fences
+// and counters, which passes beside the copies that way.
 //
-// Products: mma m16n8k16, f16 x f16 -> f32, 16 rows of the tile at a time.  The codes become f16 exactly, one conversion per
-// two codes, straight into operand registers:
-//   * which head_dim value sits at which position of the contraction is free as long as queries and keys agree, so thread
-//     (g = lane / 4, c = lane % 4) takes the D / 4 consecutive values from c * D / 4 of key g;
-//   * for P V the same freedom holds for the columns: thread g takes the D / 8 consecutive values from g * D / 8 of the keys
-//     2c, 2c + 1, 2c + 8, 2c + 9, which are the keys whose probabilities the score fragment leaves in this thread.
-// So 16-byte shared-memory loads, conflict-free under the swizzle, feed the tensor cores without any exchange.
+// Products, on the warp-level tensor instructions (an item has 1 to 32 rows; a 128-row tcgen05 tile would be empty), both
+// transposed so that keys and head dimension fill the instruction's 16 rows and 8 queries its columns:
+//   S^T = K Q^T  m16n8k32 e4m3 x e4m3 -> f32.  The keys' codes are the operand as they lie in the cache, nothing is converted;
+//                the queries are split into e4m3 terms.  (As an f16 product with converted keys, a third of all
+//                instructions were conversions.)
+//   O^T = V^T P^T  m16n8k16 f16.  The values' codes become f16 exactly, two per conversion; P^T comes from the score
+//                fragment by an 8 x 8 transpose between lanes.
+// Which head_dim value sits at which position of a contraction is free as long as both operands agree, and so is the order
+// of the result's rows: thread (g = lane / 4, c = lane % 4) takes the D / 4 consecutive values from c * D / 4 of keys g, g + 8, ..,
+// and the D / 8 consecutive values from g * D / 8 of keys 2c, 2c + 1, 2c + 8, ...  So 16-byte shared-memory loads,
+// conflict-free under the swizzle, feed the tensor cores.
 //
-// Precision.  Queries are scaled per row by a power of two to [1, 2) before they become f16 (exact but for values below
-// 2^-24 of the row's largest).  The value scale vs of a block joins the exponent, p' = 2^(score + log2 vs - m), with m the running
-// maximum of score + log2 vs, so the f16 operand holds the weight with which the block's CODES enter the sum: its largest is
-// near 1 whatever the scales, and f16's 11 bits hold (2^-12 relative error, 2^-25 absolute below 2^-14).  The softmax's
-// weight is sum p' / vs in f32.  m only moves when it would grow by more than 2^8 (p' stays far below f16's 65504).
+// Precision.  A query row is scaled by a power of two to [128, 256) and split: e4m3(q), then 16 times the rest, once for
+// bf16 and twice for f16; 4 + 4 (+ 4) significant bits hold the type's 8 (11) exactly, but for values below 2^-13 of the
+// row's largest, which keep an absolute error of 2^-21 of it.  The products are exact and added in f32.
+// The value scale vs of a block joins the exponent, p' = 2^(score + log2 vs - m), with m the running maximum of score +
+// log2 vs, so the f16 operand holds the weight with which the block's CODES enter the sum: its largest is near 1 whatever the
+// scales, and f16's 11 bits hold (2^-12 relative error, 2^-25 absolute below 2^-14).  The softmax's weight is sum p' / vs in
+// f32.  m only moves when a score exceeds it by more than 2^8 (p' stays far below f16's 65504): a vote of the warp finds
+// that out, and only then the maximum is formed across lanes and the sums are rescaled.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cuda_fp8.h>
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "internal.h"
 #include "paged_attention.cuh"
@@ -35,32 +46,51 @@ namespace {
 
 constexpr int GROUP = 32;                    // keys that a warp takes at a time
 
-// MT: 16-row tiles per item.
-template <int D, int MT>
+// NQ: 8-row query tiles per item.
+template <int D, int NQ>
 struct ShortCfg {
-    static constexpr int NW = MT == 1 ? 4 : 8;                             // warps per CTA
-    static constexpr int PER_SM = MT == 1 ? 3 : 1;                         // resident CTAs
+    static constexpr int ROWS = NQ * 8;                                    // query rows per item
+    static constexpr int NW = NQ <= 2 ? 4 : 8;                             // warps per CTA
+    static constexpr int PER_SM = NQ == 1 ? 3 : NQ == 2 ? 2 : 1;           // resident CTAs
     static constexpr int THREADS = NW * 32;
     static constexpr int UNIT = NW * GROUP;                                // keys per unit
     static constexpr int TILE = GROUP * D;                                 // bytes of a group's keys (or values)
-    static constexpr int RING_BYTES = (MT == 1 ? 64 : 192) * 1024;
+    static constexpr int RING_BYTES = (NQ == 1 ? 64 : NQ == 2 ? 96 : 192) * 1024;
     static constexpr int STAGES = RING_BYTES / (NW * 2 * TILE);
+    static constexpr int TERM_BYTES = ROWS * D;                            // one e4m3 term of the queries, in operand order
     static constexpr int Q_OFF = RING_BYTES;
-    static constexpr int Q_BYTES = MT * 16 * D * 2;
-    static constexpr int ROW_OFF = Q_OFF + Q_BYTES;                        // float [MT * 16] row scales
-    static constexpr int ML_OFF = ROW_OFF + MT * 16 * 4;                   // float [NW][MT * 16][2]
-    static constexpr int INFO_OFF = ML_OFF + NW * MT * 16 * 8;             // float4 [NW][STAGES][2]
+    static constexpr int ROW_OFF = Q_OFF + 3 * TERM_BYTES;                // float [ROWS] row scales
+    static constexpr int ML_OFF = ROW_OFF + ROWS * 4;                      // float [NW][ROWS][2]
+    static constexpr int INFO_OFF = ML_OFF + NW * ROWS * 8;                // float4 [NW][STAGES][2]
     static constexpr int BAR_OFF = INFO_OFF + NW * STAGES * 32;            // mbarriers [NW][STAGES]
-    static constexpr int MISC_OFF = BAR_OFF + NW * STAGES * 8;             // long long [NW], int flag
-    static constexpr int BYTES = MISC_OFF + NW * 8 + 16 + 1024;            // + alignment
-    static_assert(NW * MT * 16 * D * 4 <= RING_BYTES, "the ring holds the warps' sums at an item's end");
-    static_assert(STAGES >= 2 && STAGES <= 32 && (BYTES + 1024) * PER_SM <= 228 * 1024, "shared memory of an SM");
+    static constexpr int SHARES_OFF = BAR_OFF + NW * STAGES * 8;
+    static constexpr int SPLIT_OFF = SHARES_OFF + sizeof(PagedShares);     // PagedCursor [2], int [2], int [2]
+    static constexpr int BYTES = SPLIT_OFF + 2 * sizeof(PagedCursor) + 16;
+    static constexpr int EARLY = NQ <= 2 ? 1 : 0;                          // groups of the next item that are asked for before this one's sums are joined
+    static_assert(ROWS * D * 4 <= (EARLY ? 1 : STAGES) * 2 * TILE, "a warp's sums beside them");
+    static_assert(SHARES_OFF % 8 == 0 && STAGES >= 2 && STAGES <= 16 && (BYTES + 1024) * PER_SM <= 228 * 1024, "shared memory of an SM");
 };
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 8 x 8 matrix of 16-bit values, two per lane (row lane / 4, columns 2c, 2c + 1), transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
     uint4 v;
@@ -82,36 +112,108 @@ template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(ShortCfg<D, MT>::THREADS, ShortCfg<D, MT>::PER_SM)
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(ShortCfg<D, NQ>::THREADS, ShortCfg<D, NQ>::PER_SM)
 paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PagedParams p, int halves) {
-    using SM = ShortCfg<D, MT>;
+    using SM = ShortCfg<D, NQ>;
     constexpr int NW = SM::NW, THREADS = SM::THREADS, UNIT = SM::UNIT;
-    constexpr int TILE = MT * 16, S = SM::STAGES, KC = D / 64, NT = D / 8;   // KC: 16-byte chunks of a key per thread; NT: column tiles
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    constexpr int TILE = SM::ROWS, S = SM::STAGES, KC = D / 64, NT = D / 8;  // KC: 16-byte chunks of a key per thread; NT: values of a token per thread
+    constexpr int TERMS = std::is_same<T, __half>::value ? 3 : 2;
+    extern __shared__ __align__(1024) uint8_t smem[];                        // the swizzle goes by address bits: the copies' memory starts on 1024 bytes
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c4 = lane & 3;
     float* row_scale = reinterpret_cast<float*>(smem + SM::ROW_OFF);
     float* warp_ml = reinterpret_cast<float*>(smem + SM::ML_OFF);
+    PagedShares& shares = *reinterpret_cast<PagedShares*>(smem + SM::SHARES_OFF);
+    PagedCursor (&split)[2] = *reinterpret_cast<PagedCursor (*)[2]>(smem + SM::SPLIT_OFF);
+    int (&is_split)[2] = *reinterpret_cast<int (*)[2]>(smem + SM::SPLIT_OFF + 2 * sizeof(PagedCursor));
+    int* flags = reinterpret_cast<int*>(smem + SM::SPLIT_OFF + 2 * sizeof(PagedCursor) + 8);
     float4* info = reinterpret_cast<float4*>(smem + SM::INFO_OFF) + w * S * 2;
     const uint32_t bars = smem_u32(smem + SM::BAR_OFF) + w * S * 8;
     const uint32_t ring = smem_u32(smem) + w * S * 2 * SM::TILE;
-    const uint32_t q_frags = smem_u32(smem + SM::Q_OFF) + lane * 16;
-    long long* scratch = reinterpret_cast<long long*>(smem + SM::MISC_OFF);
-    int* flag = reinterpret_cast<int*>(scratch + NW);
+    const uint32_t q_frags = smem_u32(smem + SM::Q_OFF) + lane * 16;         // [term][query tile][64 values of D][lane]: 16 bytes
 
     if (lane == 0) {
         for (int i = 0; i < S; ++i) mbar_init(bars + 8 * i, halves);
         fence_barrier_init();
         fence_proxy_async();
-        if (w == 0) { prefetch_tmap(&tmK); prefetch_tmap(&tmV); }
+        if (w == 0) is_split[0] = is_split[1] = 0;
     }
     PagedCursor c;
-    const bool busy = paged_begin<THREADS, TILE, UNIT>(p, c, scratch, 1);
+    const bool busy = paged_begin<THREADS, TILE, UNIT>(p, c, shares, 1);
     __syncthreads();
     if (!busy) return;
-    uint32_t phases = 0;                     // parity of each stage's next completion
     bool ok = true;
+
+    // ---- the warp's copies.  A group lies in one block (halves = 1, block sizes from 32) or in two of 16 tokens (halves = 2).  Lane
+    // unit * halves + half, counted from unit `base`, has the id and scales of one of them and issues its copies.
+    const int mine_u = halves == 2 ? lane >> 1 : lane, mine_h = halves == 2 ? lane & 1 : 0;
+    int base = 0, id = -1;                   // block (-1: masked)
+    float ks = 0.0f, vs = 1.0f;              // its scales as loaded
+    float4 about;                            // key scale (0: masked), log2 of the value scale, 1 / it
+    auto block_of = [&](const PagedCursor& at, int j, int j1, int kend) {    // asked for; the caller checks its range
+        const int key = (j + mine_u) * UNIT + w * GROUP + mine_h * 16;
+        return j + mine_u < j1 && key < kend ? __ldg(p.table + static_cast<size_t>(at.r) * p.max_blocks + (key >> p.shift)) : -1;
+    };
+    auto take = [&](int j, int block) { base = j; id = static_cast<unsigned>(block) < static_cast<unsigned>(p.num_blocks) ? block : -1; };
+    auto scales = [&]() {                    // asked for; `describe` waits for them
+        ks = 0.0f; vs = 1.0f;
+        if (id >= 0) {
+            const size_t at = static_cast<size_t>(id) * p.kv_heads + c.h;
+            ks = __ldg(p.k_scale + at); vs = __ldg(p.v_scale + at);
+        }
+    };
+    auto describe = [&]() {
+        vs = paged_clamp_scale(vs);
+        about = make_float4(id >= 0 ? paged_clamp_scale(ks) : 0.0f, log2f(vs), 1.0f / vs, 0.0f);
+    };
+    auto copy = [&](int j, uint32_t at) {    // unit j's group into stage `at`; all lanes call it
+        if (mine_u == j - base) {
+            if (id >= 0) {
+                const uint32_t bytes = SM::TILE / halves, dst = ring + at * 2 * SM::TILE + mine_h * (SM::TILE / 2);
+                const int y = ((j * UNIT + w * GROUP + mine_h * 16) & (p.block_size - 1)) * D / 128, z = id * p.kv_heads + c.h;
+                mbar_arrive_expect_tx(bars + 8 * at, 2 * bytes);
+                tma_load_3d(dst, &tmK, bars + 8 * at, 0, y, z);
+                tma_load_3d(dst + SM::TILE, &tmV, bars + 8 * at, 0, y, z);
+            } else mbar_arrive(bars + 8 * at);
+        }
+    };
+    auto note = [&](int j, uint32_t at) {    // what the products have to know about it
+        if (mine_u == j - base) {
+            info[at * 2 + mine_h] = about;
+            if (halves == 1) info[at * 2 + 1] = about;
+        }
+    };
+    uint32_t st = 0, parity = 0;             // stage that is read next, parity of its completion
+    auto stage = [&](int i) { const uint32_t at = st + i; return at >= S ? at - S : at; };   // i < S stages on
+    // ---- the queries: 16 threads per row, D / 16 values each; loaded an item ahead
+    constexpr int PARTS = (TILE * 16 + THREADS - 1) / THREADS, NV = D / 16;
+    uint32_t q_raw[PARTS][NV / 2];
+    auto load_q = [&](const PagedCursor& at) {
+        const int row0 = at.t * TILE, rows = min(TILE, at.q.rows - row0);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+            const int row = part * (THREADS / 16) + (threadIdx.x >> 4), x = threadIdx.x & 15;
+#pragma unroll
+            for (int i = 0; i < NV / 2; ++i) q_raw[part][i] = 0;
+            if (row < rows) {
+                const int token = (row0 + row) / p.group, head = at.h * p.group + (row0 + row - token * p.group);
+                const T* src = static_cast<const T*>(p.q) + (static_cast<size_t>(at.q.start) + token) * p.q_stride + static_cast<size_t>(head) * D + x * NV;
+                if constexpr (NV == 8) { const uint4 v = __ldg(reinterpret_cast<const uint4*>(src)); q_raw[part][0] = v.x; q_raw[part][1] = v.y; q_raw[part][2] = v.z; q_raw[part][3] = v.w; }
+                else { const uint2 v = __ldg(reinterpret_cast<const uint2*>(src)); q_raw[part][0] = v.x; q_raw[part][1] = v.y; }
+            }
+        }
+    };
+
+    int ahead;                               // block of the next item's first groups
+    {
+        const int j0 = c.from(), j1 = c.to();
+        take(j0, block_of(c, j0, j1, paged_tile_end<TILE>(p, c.q, c.t)));
+        load_q(c);
+#pragma unroll 1
+        for (int i = 0; i < S && j0 + i < j1; ++i) copy(j0 + i, i);
+        scales();
+    }
+
     // this thread's places in a stage: keys g (+ 8, 16, 24) and values 2c, 2c + 1 (+ 8, ...).  8 lines on the swizzle repeats: that
     // is 8 keys for D = 128 and 16 for D = 64, where 8 keys on the chunk's bit 2 (64 bytes) is the other one
     constexpr int ODD = D == 64 ? 64 : 0;
@@ -121,337 +223,314 @@ paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 #pragma unroll
     for (int i = 0; i < 2; ++i) { v_at[i][0] = swizzled((2 * c4 + i) * D + g * NT); v_at[i][1] = v_at[i][0] ^ ODD; }
 
-    for (long long u = c.lo; u < c.hi;) {
-        const int j0 = static_cast<int>(u - c.item), j1 = static_cast<int>(min(static_cast<long long>(c.units), c.hi - c.item));
+    for (;;) {
+        const int j0 = c.from(), j1 = c.to();
         const int row0 = c.t * TILE, rows = min(TILE, c.q.rows - row0);
         const int kend = paged_tile_end<TILE>(p, c.q, c.t);
-        const int* table = p.table + static_cast<size_t>(c.r) * p.max_blocks;
 
-        // ---- the ring.  A group lies in one block (halves = 1, block sizes from 32) or in two of 16 tokens (halves = 2).  Lane
-        // (j - base) * halves + i holds id and scales of half i of unit j's group, and issues its copies.
-        int base = j0, id = -1;
-        float4 about = make_float4(0.0f, 0.0f, 1.0f, 0.0f);                  // key scale (0: masked), log2 of the value scale, 1 / it
-        auto fetch = [&](int j) {
-            base = j;
-            const int mine = j + (halves == 2 ? lane >> 1 : lane);
-            const long long key = static_cast<long long>(mine) * UNIT + w * GROUP + (halves == 2 ? (lane & 1) * 16 : 0);
-            id = -1;
-            if (mine < j1 && key < kend) {
-                id = __ldg(table + (key >> p.shift));
-                if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.num_blocks)) id = -1;
-            }
-            about.x = 0.0f;
-            if (id >= 0) {
-                const size_t at = static_cast<size_t>(id) * p.kv_heads + c.h;
-                const float vs = paged_clamp_scale(__ldg(p.v_scale + at));
-                about = make_float4(paged_clamp_scale(__ldg(p.k_scale + at)), log2f(vs), 1.0f / vs, 0.0f);
-            }
-        };
-        auto issue = [&](int j, int st) {    // warp-uniform
-            if (j >= j1 || !ok) return;
-            if ((j - base) * halves >= 32) fetch(j);
-            const int i = lane - (j - base) * halves;
-            if (i >= 0 && i < halves) {
-                info[st * 2 + i] = about;
-                if (halves == 1) info[st * 2 + 1] = about;
-                if (id >= 0) {
-                    const uint32_t bytes = SM::TILE / halves, dst = ring + st * 2 * SM::TILE + i * (SM::TILE / 2);
-                    const int y = ((j * UNIT + w * GROUP + i * 16) & (p.block_size - 1)) * D / 128, z = id * p.kv_heads + c.h;
-                    mbar_arrive_expect_tx(bars + 8 * st, 2 * bytes);
-                    tma_load_3d(dst, &tmK, bars + 8 * st, 0, y, z);
-                    tma_load_3d(dst + SM::TILE, &tmV, bars + 8 * st, 0, y, z);
-                } else mbar_arrive(bars + 8 * st);
-            }
-        };
-        fetch(j0);
-#pragma unroll 1
-        for (int i = 0; i < S; ++i) issue(j0 + i, i);
-
-        // ---- queries to f16 operand order: 16 threads per row, D / 16 values each
+        // ---- queries to e4m3 terms in operand order
 #pragma unroll
-        for (int part = 0; part < TILE * 16 / THREADS; ++part) {
-            const int row = part * (THREADS / 16) + (threadIdx.x >> 4), mt = row >> 4, x = threadIdx.x & 15;
-            constexpr int NV = D / 16;
+        for (int part = 0; part < PARTS; ++part) {
+            const int row = part * (THREADS / 16) + (threadIdx.x >> 4), x = threadIdx.x & 15;
             float v[NV];
             float amax = 0.0f;
             bool finite = true;
-            if (row < rows) {
-                const int token = (row0 + row) / p.group, head = c.h * p.group + (row0 + row - token * p.group);
-                const T* src = static_cast<const T*>(p.q) + (static_cast<size_t>(c.q.start) + token) * p.q_stride + static_cast<size_t>(head) * D + x * NV;
-                uint32_t wd[NV / 2];
-                if constexpr (NV == 8) *reinterpret_cast<uint4*>(wd) = __ldg(reinterpret_cast<const uint4*>(src));
-                else *reinterpret_cast<uint2*>(wd) = __ldg(reinterpret_cast<const uint2*>(src));
 #pragma unroll
-                for (int i = 0; i < NV / 2; ++i) {
-                    const float2 f = unpack2<T>(wd[i]);
-                    v[2 * i] = f.x; v[2 * i + 1] = f.y;
-                    amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-                    finite &= fabsf(f.x) < INFINITY && fabsf(f.y) < INFINITY;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < NV; ++i) v[i] = 0.0f;
+            for (int i = 0; i < NV / 2; ++i) {
+                const float2 f = unpack2<T>(q_raw[part][i]);
+                v[2 * i] = f.x; v[2 * i + 1] = f.y;
+                amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+                finite &= fabsf(f.x) < INFINITY && fabsf(f.y) < INFINITY;
             }
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o, 16));
             const unsigned all = __ballot_sync(0xffffffffu, finite);
             const bool row_finite = ((all >> (lane & 16)) & 0xffffu) == 0xffffu;
-            // 2^-e brings the largest to [1, 2) (at the ends of the range, where 2^e or 2^-e would be subnormal, within [0, 4))
-            const int e = amax > 0.0f && row_finite ? min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -126), 126) : 0;
+            // 2^-e brings the largest to [128, 256) (below 2^-119, where 2^-e leaves the range, to less)
+            const int e = amax > 0.0f && row_finite ? max(static_cast<int>(__float_as_uint(amax) >> 23) - 134, -126) : 0;
             const float down = exp2_int(-e);
-            if (x == 0) row_scale[row] = row_finite ? exp2_int(e) * p.scale_log2 : __int_as_float(0x7fffffff);
-            const int r16 = row & 15;
+            if (row < TILE) {
+                if (x == 0) row_scale[row] = row_finite ? exp2_int(e) * p.scale_log2 : __int_as_float(0x7fffffff);
+                float f[NV];
 #pragma unroll
-            for (int i = 0; i < NV; i += 2) {
-                const int d = x * NV + i;
-                const int cc = d / (D / 4), j = (d % (D / 4)) / 4, pos = d & 3;
-                const __half2 h = __floats2half2_rn(v[i] * down, v[i + 1] * down);
-                const int reg = (r16 >= 8 ? 1 : 0) + (pos >= 2 ? 2 : 0);
-                *reinterpret_cast<__half2*>(smem + SM::Q_OFF + ((((mt * (D / 16) + j) * 32) + (r16 & 7) * 4 + cc) * 4 + reg) * 4) = h;
+                for (int i = 0; i < NV; ++i) f[i] = row_finite ? v[i] * down : 0.0f;
+                // operand position of values d .. d + 3 (d = 4 * word of thread c's D / 4): chunk of 16 values, then word
+#pragma unroll
+                for (int i = 0; i < NV; i += 4) {
+                    const int d = x * NV + i, cc = d / (D / 4), word = (d % (D / 4)) / 4;
+                    uint8_t* dst = smem + SM::Q_OFF + (((row >> 3) * KC + word / 4) * 32 + (row & 7) * 4 + cc) * 16 + (word & 3) * 4;
+#pragma unroll
+                    for (int term = 0; term < TERMS; ++term) {
+                        const uint32_t q4 = e4m3x4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+                        *reinterpret_cast<uint32_t*>(dst + term * SM::TERM_BYTES) = q4;
+                        const float2 lo = e4m3x2_to_float2(q4 & 0xffffu), hi = e4m3x2_to_float2(q4 >> 16);
+                        const float up = term == 0 ? 16.0f : 1.0f;           // the rests share one scale and one accumulator
+                        f[i] = (f[i] - lo.x) * up; f[i + 1] = (f[i + 1] - lo.y) * up; f[i + 2] = (f[i + 2] - hi.x) * up; f[i + 3] = (f[i + 3] - hi.y) * up;
+                    }
+                }
             }
+        }
+        describe();
+#pragma unroll 1
+        for (int i = 0; i < S && j0 + i < j1; ++i) note(j0 + i, stage(i));
+        const bool more = c.more();
+        ahead = -1;
+        if (more) {                          // what the next item begins with
+            PagedCursor then = c;
+            paged_next<TILE, UNIT>(p, then);
+            ahead = block_of(then, 0, then.to(), paged_tile_end<TILE>(p, then.q, then.t));
+            load_q(then);
         }
         __syncthreads();
 
-        int lim[MT][2];
-        float qs[MT][2];
+        // this thread's queries: 2c and 2c + 1 of every tile
+        int lim[NQ][2];
+        float qs[NQ][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int t = 0; t < NQ; ++t)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int row = mt * 16 + i * 8 + g;
-                lim[mt][i] = row < rows ? paged_limit(p, c.q, (row0 + row) / p.group) : kend;
-                qs[mt][i] = row_scale[row];
+                const int row = t * 8 + 2 * c4 + i;
+                lim[t][i] = row < rows ? paged_limit(p, c.q, (row0 + row) / p.group) : kend;
+                qs[t][i] = row_scale[row];
             }
         const int all_see = paged_limit(p, c.q, row0 / p.group);             // keys that every row sees
 
-        float o[MT][NT][4], m[MT][2], l[MT][2];
+        float o[NQ][D / 16][4], m[NQ][2], l[NQ][2];                          // o: values g * NT + 2n (0, 1) and + 1 (2, 3) of the two queries
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int t = 0; t < NQ; ++t) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) { m[mt][i] = -INFINITY; l[mt][i] = 0.0f; }
+            for (int i = 0; i < 2; ++i) { m[t][i] = -INFINITY; l[t][i] = 0.0f; }
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < D / 16; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[mt][n][i] = 0.0f;
+                for (int i = 0; i < 4; ++i) o[t][n][i] = 0.0f;
         }
 
-        int st = 0;
 #pragma unroll 1
         for (int j = j0; j < j1; ++j) {
-            __syncwarp();
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bars + 8 * st, parity, p.status, 0x61));
             const float4 in0 = info[st * 2], in1 = info[st * 2 + 1];
-            if (ok) {
-                ok = __all_sync(0xffffffffu, mbar_wait(bars + 8 * st, (phases >> st) & 1, p.status, 0x61));
-                phases ^= 1u << st;
+            const uint32_t kt = ring + st * 2 * SM::TILE, vt = kt + SM::TILE;
+            const int key0 = j * UNIT + w * GROUP;
+            // scores of keys g, g + 8, g + 16, g + 24 with this thread's queries: s[tile][key group of 16][key 0/8, query 0/1]
+            float s[NQ][2][4], r[NQ][2][4];
+#pragma unroll
+            for (int t = 0; t < NQ; ++t)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { s[t][k][i] = 0.0f; r[t][k][i] = 0.0f; }
+#pragma unroll
+            for (int i = 0; i < KC; ++i) {
+                uint4 kk[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) kk[t] = lds128(kt + k_at[i][t & 1] + t * 8 * D);
+#pragma unroll
+                for (int t = 0; t < NQ; ++t)
+#pragma unroll
+                    for (int term = 0; term < TERMS; ++term) {
+                        const uint4 q = lds128(q_frags + term * SM::TERM_BYTES + (t * KC + i) * 512);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            float (&acc)[4] = term == 0 ? s[t][k] : r[t][k];
+                            mma_e4m3(acc, kk[2 * k].x, kk[2 * k + 1].x, kk[2 * k].y, kk[2 * k + 1].y, q.x, q.y);
+                            mma_e4m3(acc, kk[2 * k].z, kk[2 * k + 1].z, kk[2 * k].w, kk[2 * k + 1].w, q.z, q.w);
+                        }
+                    }
             }
-            if (ok && (in0.x > 0.0f || in1.x > 0.0f)) {
-                const uint32_t kt = ring + st * 2 * SM::TILE;
-                const int key0 = j * UNIT + w * GROUP;
-                float s[MT][4][4];
+            const bool cut = key0 + GROUP > all_see || in0.x == 0.0f || in1.x == 0.0f;          // some row does not see some key of the group
+            uint32_t pb[NQ][4];                                              // P^T operands of 8 keys each
+            bool above = false;
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+            for (int t = 0; t < NQ; ++t) {
 #pragma unroll
-                    for (int t = 0; t < 4; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[mt][t][i] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < KC; ++i) {
-                    uint4 kk[4];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) kk[t] = lds128(kt + k_at[i][t & 1] + t * 8 * D);
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        uint32_t b[4][2];
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) e4m3x4_to_f16x4(x == 0 ? kk[t].x : x == 1 ? kk[t].y : x == 2 ? kk[t].z : kk[t].w, b[t][0], b[t][1]);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            const uint4 qa = lds128(q_frags + (mt * (D / 16) + i * 4 + x) * 512);
-                            const uint32_t a[4] = {qa.x, qa.y, qa.z, qa.w};
-#pragma unroll
-                            for (int t = 0; t < 4; ++t) mma_f16(s[mt][t], a, b[t][0], b[t][1]);
-                        }
-                    }
-                }
-                const bool cut = key0 + GROUP > all_see || in0.x == 0.0f || in1.x == 0.0f;      // some row does not see some key of the group
-                uint32_t pa[MT][2][4];
-                bool moved = false;
-                float alpha[MT][2];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float f0 = qs[mt][i] * in0.x, f1 = qs[mt][i] * in1.x;
-                        float x[8];
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            x[2 * t] = fmaf(s[mt][t][2 * i], t < 2 ? f0 : f1, t < 2 ? in0.y : in1.y);
-                            x[2 * t + 1] = fmaf(s[mt][t][2 * i + 1], t < 2 ? f0 : f1, t < 2 ? in0.y : in1.y);
-                        }
-                        if (cut) {
-                            const int left = lim[mt][i] - key0 - 2 * c4;
-#pragma unroll
-                            for (int t = 0; t < 4; ++t) {
-                                const bool gone = (t < 2 ? in0.x : in1.x) == 0.0f;
-                                if (gone || t * 8 >= left) x[2 * t] = -INFINITY;
-                                if (gone || t * 8 + 1 >= left) x[2 * t + 1] = -INFINITY;
-                            }
-                        }
-                        float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                        const bool move = mx > m[mt][i] + 8.0f;              // also from -inf
-                        alpha[mt][i] = move ? ex2_approx(m[mt][i] - mx) : 1.0f;
-                        if (move) m[mt][i] = mx;
-                        moved |= move;
-                        const float ref = m[mt][i] == -INFINITY ? 0.0f : m[mt][i];
-#pragma unroll
-                        for (int t = 0; t < 8; ++t) x[t] = ex2_approx(x[t] - ref);
-                        l[mt][i] = fmaf((x[0] + x[1]) + (x[2] + x[3]), in0.z, fmaf((x[4] + x[5]) + (x[6] + x[7]), in1.z, l[mt][i] * alpha[mt][i]));
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            const __half2 h = __floats2half2_rn(x[2 * t], x[2 * t + 1]);
-                            pa[mt][t >> 1][(t & 1) * 2 + i] = *reinterpret_cast<const uint32_t*>(&h);
-                        }
-                    }
-                }
-                if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) o[mt][n][i] *= alpha[mt][i >> 1];
-                }
-                // values, 16 keys at a time: rows 2c, 2c + 1, 2c + 8, 2c + 9, D / 8 codes each
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t v[4][NT / 4];
+                for (int k = 0; k < 2; ++k)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint32_t a = kt + SM::TILE + v_at[i & 1][i >> 1] + (half * 16 + (i >> 1) * 8) * D;
-                        if constexpr (NT == 16) { const uint4 x = lds128(a); v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w; }
-                        else { const uint2 x = lds64(a); v[i][0] = x.x; v[i][1] = x.y; }
+                        const float f = qs[t][i & 1] * (k ? in1.x : in0.x);
+                        s[t][k][i] = fmaf(fmaf(r[t][k][i], 0.0625f, s[t][k][i]), f, k ? in1.y : in0.y);
                     }
-                    bool own_nan = false;
-                    if (cut) {
-                        const bool gone = (half ? in1.x : in0.x) == 0.0f;
-                        uint32_t nans = 0;
+                if (cut) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const bool past = gone || key0 + half * 16 + 2 * c4 + (i & 1) + (i >> 1) * 8 >= kend;
+                    for (int k = 0; k < 2; ++k)
 #pragma unroll
-                            for (int x = 0; x < NT / 4; ++x) {
-                                if (past) v[i][x] = 0;                       // behind the last key of the tile: whatever is there
-                                const uint32_t z = nan_codes(v[i][x]);
-                                nans |= z;
-                                v[i][x] &= ~((z >> 7) * 0xffu);              // 0 * NaN would reach the rows that do not see it
-                            }
+                        for (int i = 0; i < 4; ++i)
+                            if ((k ? in1.x : in0.x) == 0.0f || key0 + k * 16 + (i >> 1) * 8 + g >= lim[t][i & 1]) s[t][k][i] = -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) above |= fmaxf(fmaxf(s[t][0][i], s[t][0][2 + i]), fmaxf(s[t][1][i], s[t][1][2 + i])) > m[t][i] + 8.0f;   // also from -inf
+            }
+            if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+                for (int t = 0; t < NQ; ++t) {
+                    float alpha[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float mx = fmaxf(fmaxf(s[t][0][i], s[t][0][2 + i]), fmaxf(s[t][1][i], s[t][1][2 + i]));
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                        const bool move = mx > m[t][i] + 8.0f;
+                        alpha[i] = move ? ex2_approx(m[t][i] - mx) : 1.0f;
+                        if (move) m[t][i] = mx;
+                        l[t][i] *= alpha[i];
+                    }
+#pragma unroll
+                    for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[t][n][i] *= alpha[i & 1];
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NQ; ++t) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float ref = m[t][i] == -INFINITY ? 0.0f : m[t][i];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) { s[t][k][i] = ex2_approx(s[t][k][i] - ref); s[t][k][2 + i] = ex2_approx(s[t][k][2 + i] - ref); }
+                    l[t][i] = fmaf(s[t][0][i] + s[t][0][2 + i], in0.z, fmaf(s[t][1][i] + s[t][1][2 + i], in1.z, l[t][i]));
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const __half2 h = __floats2half2_rn(s[t][k >> 1][(k & 1) * 2], s[t][k >> 1][(k & 1) * 2 + 1]);
+                    pb[t][k] = transpose8(*reinterpret_cast<const uint32_t*>(&h));
+                }
+            }
+            // values, 16 keys at a time: keys 2c, 2c + 1, 2c + 8, 2c + 9, D / 8 codes each
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t v[4][NT / 4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t a = vt + v_at[i & 1][i >> 1] + (half * 16 + (i >> 1) * 8) * D;
+                    if constexpr (NT == 16) { const uint4 x = lds128(a); v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w; }
+                    else { const uint2 x = lds64(a); v[i][0] = x.x; v[i][1] = x.y; }
+                }
+                bool own_nan = false;
+                if (cut) {
+                    const bool gone = (half ? in1.x : in0.x) == 0.0f;
+                    uint32_t nans = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool past = gone || key0 + half * 16 + 2 * c4 + (i & 1) + (i >> 1) * 8 >= kend;
+#pragma unroll
+                        for (int x = 0; x < NT / 4; ++x) {
+                            if (past) v[i][x] = 0;                       // behind the last key of the tile: whatever is there
+                            const uint32_t z = nan_codes(v[i][x]);
+                            nans |= z;
+                            v[i][x] &= ~((z >> 7) * 0xffu);              // 0 * NaN would reach the rows that do not see it
                         }
-                        own_nan = __any_sync(0xffffffffu, nans != 0);
                     }
+                    own_nan = __any_sync(0xffffffffu, nans != 0);
+                }
 #pragma unroll
-                    for (int x = 0; x < NT / 4; ++x) {
-                        // bytes of two keys side by side: (key, key + 1) for columns 4x, 4x + 1 | 4x + 2, 4x + 3
-                        uint32_t b0[4], b1[4];
-                        e4m3x4_to_f16x4(prmt(v[0][x], v[1][x], 0x5140), b0[0], b0[1]);
-                        e4m3x4_to_f16x4(prmt(v[0][x], v[1][x], 0x7362), b0[2], b0[3]);
-                        e4m3x4_to_f16x4(prmt(v[2][x], v[3][x], 0x5140), b1[0], b1[1]);
-                        e4m3x4_to_f16x4(prmt(v[2][x], v[3][x], 0x7362), b1[2], b1[3]);
+                for (int x = 0; x < NT / 4; ++x) {
+                    // bytes of two keys side by side: (key, key + 1) for values 4x, 4x + 1 | 4x + 2, 4x + 3
+                    uint32_t a[4], b[4];
+                    e4m3x4_to_f16x4(prmt(v[0][x], v[1][x], 0x5140), a[0], a[1]);
+                    e4m3x4_to_f16x4(prmt(v[0][x], v[1][x], 0x7362), a[2], a[3]);
+                    e4m3x4_to_f16x4(prmt(v[2][x], v[3][x], 0x5140), b[0], b[1]);
+                    e4m3x4_to_f16x4(prmt(v[2][x], v[3][x], 0x7362), b[2], b[3]);
 #pragma unroll
-                        for (int y = 0; y < 4; ++y)
-#pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][4 * x + y], pa[mt][half], b0[y], b1[y]);
+                    for (int t = 0; t < NQ; ++t) {
+                        mma_f16(o[t][2 * x], a[0], a[1], b[0], b[1], pb[t][2 * half], pb[t][2 * half + 1]);
+                        mma_f16(o[t][2 * x + 1], a[2], a[3], b[2], b[3], pb[t][2 * half], pb[t][2 * half + 1]);
                     }
-                    if (own_nan) {                                           // NaN values in a group that not every row sees whole: only to the rows that see them
-                        for (int k = 0; k < 16; ++k) {
-                            const int key = key0 + half * 16 + k;
-                            if (key >= kend) break;
+                }
+                if (own_nan) {                                           // NaN values in a group that not every row sees whole: only to the rows that see them
+                    for (int k = 0; k < 16; ++k) {
+                        const int key = key0 + half * 16 + k;
+                        if (key >= kend) break;
 #pragma unroll
-                            for (int n = 0; n < NT; ++n)
+                        for (int n = 0; n < NT; ++n) {
+                            uint32_t byte;
+                            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(vt + swizzled((half * 16 + k) * D + g * NT + n)));
+                            if ((byte & 127u) == 127u) {
 #pragma unroll
-                                for (int y = 0; y < 2; ++y) {
-                                    uint32_t byte;
-                                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(kt + SM::TILE + swizzled((half * 16 + k) * D + (2 * c4 + y) * NT + n)));
-                                    if ((byte & 127u) == 127u) {
+                                for (int t = 0; t < NQ; ++t)
 #pragma unroll
-                                        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                                            for (int i = 0; i < 2; ++i)
-                                                if (key < lim[mt][i]) o[mt][n][2 * i + y] = __int_as_float(0x7fffffff);
-                                    }
-                                }
+                                    for (int i = 0; i < 2; ++i)
+                                        if (key < lim[t][i]) o[t][n >> 1][(n & 1) * 2 + i] = __int_as_float(0x7fffffff);
+                            }
                         }
                     }
                 }
             }
             __syncwarp();
-            issue(j + S, st);
-            st = st + 1 == S ? 0 : st + 1;
+            if (ok && j + S < j1) {
+                if ((j + S - base) * halves >= 32) { take(j + S, block_of(c, j + S, j1, kend)); scales(); describe(); }
+                copy(j + S, st);
+                note(j + S, st);
+            }
+            __syncwarp();
+            if (++st == S) { st = 0; parity ^= 1; }
         }
 
-        // ---- the item's end: the warps' sums meet in the ring's memory (all copies have landed and been read)
+        // ---- the item's end: the next item's first groups, then the warps' sums, which meet in the memory of later groups
+        const PagedCursor done = c;
+        if (more) {
+            paged_next<TILE, UNIT>(p, c);
+            take(0, ahead);
+            if (ok && SM::EARLY) copy(0, st);
+            scales();
+        }
+        constexpr int SUM_STRIDE = S * 2 * SM::TILE / 4;                     // floats between two warps' rings
+        float* sums = reinterpret_cast<float*>(smem) + (SM::EARLY ? stage(1) * (2 * SM::TILE / 4) : 0);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int t = 0; t < NQ; ++t)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                l[mt][i] += __shfl_xor_sync(0xffffffffu, l[mt][i], 1);
-                l[mt][i] += __shfl_xor_sync(0xffffffffu, l[mt][i], 2);
-            }
-        __syncthreads();
-        float* sums = reinterpret_cast<float*>(smem);                        // [NW][TILE][D]
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int row = mt * 16 + i * 8 + g;
+                for (int x = 4; x < 32; x <<= 1) l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], x);
+                const int row = t * 8 + 2 * c4 + i;
                 if (row < rows) {
-                    float* dst = sums + (static_cast<size_t>(w) * TILE + row) * D + 2 * c4 * NT;
+                    if (g == 0) { warp_ml[(w * TILE + row) * 2] = m[t][i]; warp_ml[(w * TILE + row) * 2 + 1] = l[t][i]; }
+                    float* dst = sums + w * SUM_STRIDE + row * D + g * NT;
 #pragma unroll
-                    for (int y = 0; y < 2; ++y)
-#pragma unroll
-                        for (int n = 0; n < NT; n += 4)
-                            *reinterpret_cast<float4*>(dst + y * NT + n) = make_float4(o[mt][n][2 * i + y], o[mt][n + 1][2 * i + y], o[mt][n + 2][2 * i + y], o[mt][n + 3][2 * i + y]);
-                    if (c4 == 0) { warp_ml[(w * TILE + row) * 2] = m[mt][i]; warp_ml[(w * TILE + row) * 2 + 1] = l[mt][i]; }
+                    for (int n = 0; n < D / 16; n += 2)
+                        *reinterpret_cast<float4*>(dst + 2 * n) = make_float4(o[t][n][i], o[t][n][2 + i], o[t][n + 1][i], o[t][n + 1][2 + i]);
                 }
             }
         __syncthreads();
-        const bool whole = j0 == 0 && j1 == c.units;
+        const bool whole = j0 == 0 && j1 == done.units;
         float* part = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + (j0 == 0 ? 1 : 0)) * (static_cast<size_t>(TILE) * (D + 2));
-        for (int e = threadIdx.x; e < rows * (D / 2); e += THREADS) {
-            const int row = e / (D / 2), d = (e % (D / 2)) * 2;
+        for (int e = threadIdx.x; e < rows * (D / 4); e += THREADS) {
+            const int row = e / (D / 4), d = (e % (D / 4)) * 4;
             float mx = -INFINITY;
 #pragma unroll
             for (int i = 0; i < NW; ++i) mx = fmaxf(mx, warp_ml[(i * TILE + row) * 2]);
             const float ref = mx == -INFINITY ? 0.0f : mx;
-            float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+            float sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
                 const float f = ex2_approx(warp_ml[(i * TILE + row) * 2] - ref);
-                const float2 x = *reinterpret_cast<const float2*>(sums + (static_cast<size_t>(i) * TILE + row) * D + d);
+                const float4 y = *reinterpret_cast<const float4*>(sums + i * SUM_STRIDE + row * D + d);
                 sum = fmaf(warp_ml[(i * TILE + row) * 2 + 1], f, sum);
-                o0 = fmaf(x.x, f, o0); o1 = fmaf(x.y, f, o1);
+                v[0] = fmaf(y.x, f, v[0]); v[1] = fmaf(y.y, f, v[1]); v[2] = fmaf(y.z, f, v[2]); v[3] = fmaf(y.w, f, v[3]);
             }
-            if (whole) paged_finish2<T, D>(p, c, row0 + row, d, o0, o1, ref, sum);
+            if (whole) paged_finish<T, D>(p, done, row0 + row, d, v, ref, sum);
             else {
-                __stcg(reinterpret_cast<float2*>(part + row * D + d), make_float2(o0, o1));
+                __stcg(reinterpret_cast<float4*>(part + row * D + d), make_float4(v[0], v[1], v[2], v[3]));
                 if (d == 0) { __stcg(part + TILE * D + row, mx); __stcg(part + TILE * (D + 1) + row, sum); }
             }
         }
+        if (!whole && threadIdx.x == 0) { split[j0 == 0 ? 1 : 0] = done; is_split[j0 == 0 ? 1 : 0] = 1; }
+        if (!more) break;
+        fence_proxy_async();                                                 // the sums' memory goes back to the copies
         __syncthreads();
-        if (!whole) paged_join<T, D, THREADS, TILE>(p, c, rows, row0, sums, flag);
-        fence_proxy_async();                                                 // the ring's memory goes back to the copies
-        __syncthreads();
-        u = c.item + j1;
-        if (u < c.hi) paged_next<TILE, UNIT>(p, c);
+        if (ok) {
+#pragma unroll 1
+            for (int i = SM::EARLY; i < S && i < c.to(); ++i) copy(i, stage(i));
+        }
     }
+    paged_announce<T, D, THREADS, TILE>(p, shares, split, is_split, flags, reinterpret_cast<float*>(smem));
     if (!ok) for (int i = 0; i < 2000; ++i) __nanosleep(1000);               // a wait has run out: let what is in flight land
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D, int NQ>
 int launch_short(const CUtensorMap& tmK, const CUtensorMap& tmV, const PagedParams& p, int halves, cudaStream_t s) {
-    using SM = ShortCfg<D, MT>;
-    auto kernel = paged_short_kernel<T, D, MT>;
+    using SM = ShortCfg<D, NQ>;
+    auto kernel = paged_short_kernel<T, D, NQ>;
     B200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES));
     kernel<<<sm_count() * SM::PER_SM, SM::THREADS, SM::BYTES, s>>>(tmK, tmV, p, halves);
     B200_CUDA_OK(cudaGetLastError());
@@ -461,9 +540,10 @@ int launch_short(const CUtensorMap& tmK, const CUtensorMap& tmV, const PagedPara
 
 constexpr size_t WS_COUNTERS = 4096;          // bytes: one int per CTA, at most 1024
 
-// Two slots of [rows][D + 2] floats per CTA, for the larger of the two forms (one or two 16-row tiles).
+// Two slots of [rows][D + 2] floats per CTA, for the largest of the forms.
 size_t partial_bytes(int head_dim) {
-    const int rows = std::max(ShortCfg<64, 1>::PER_SM * 16, ShortCfg<64, 2>::PER_SM * 32);
+    const int rows = std::max({ShortCfg<64, 1>::PER_SM * ShortCfg<64, 1>::ROWS, ShortCfg<64, 2>::PER_SM * ShortCfg<64, 2>::ROWS,
+                               ShortCfg<64, 4>::PER_SM * ShortCfg<64, 4>::ROWS});
     return static_cast<size_t>(sm_count()) * rows * 2 * (head_dim + 2) * sizeof(float);
 }
 
@@ -490,6 +570,7 @@ int pyc_b200_paged_attention(const pyc_b200_paged_attention_args* a, void* works
     if (a->requests < 1 || a->requests > 16384 || a->max_query < 1 || a->num_blocks < 1 || a->max_blocks < 1) {
         set_error("paged attention: requests (1 .. 16384), max_query, num_blocks and max_blocks must be positive"); return -1;
     }
+    if (!(a->scale > 0.0f && a->scale < INFINITY)) { set_error("paged attention: scale must be positive and finite"); return -1; }
     if (a->kv_heads < 1 || a->heads < 1 || a->heads % a->kv_heads) { set_error("paged attention: %d heads over %d key heads", a->heads, a->kv_heads); return -1; }
     if (static_cast<long long>(a->num_blocks) * a->kv_heads > INT_MAX || static_cast<long long>(a->max_blocks) * a->block_size > INT_MAX ||
         static_cast<long long>(a->max_query) * (a->heads / a->kv_heads) > INT_MAX / 2) {
@@ -524,10 +605,10 @@ int pyc_b200_paged_attention(const pyc_b200_paged_attention_args* a, void* works
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const long long most = static_cast<long long>(a->max_query) * p.group;
     p.rows_above = 0; p.rows_upto = INT_MAX;
-    const bool wide = most > 16, half = a->dtype == PYC_DTYPE_F16;
-#define B200_SHORT(D, MT) (half ? launch_short<__half, D, MT>(tmK, tmV, p, halves, s) : launch_short<__nv_bfloat16, D, MT>(tmK, tmV, p, halves, s))
-    if (a->head_dim == 128) return wide ? B200_SHORT(128, 2) : B200_SHORT(128, 1);
-    return wide ? B200_SHORT(64, 2) : B200_SHORT(64, 1);
+    const bool half = a->dtype == PYC_DTYPE_F16;
+#define B200_SHORT(D, NQ) (half ? launch_short<__half, D, NQ>(tmK, tmV, p, halves, s) : launch_short<__nv_bfloat16, D, NQ>(tmK, tmV, p, halves, s))
+    if (a->head_dim == 128) return most <= 8 ? B200_SHORT(128, 1) : most <= 16 ? B200_SHORT(128, 2) : B200_SHORT(128, 4);
+    return most <= 8 ? B200_SHORT(64, 1) : most <= 16 ? B200_SHORT(64, 2) : B200_SHORT(64, 4);
 #undef B200_SHORT
 }
 

@@ -3,10 +3,11 @@
 //
 // Work.  An ITEM is (request, tile of query rows, key head): the rows are the request's queries times the query heads of
 // that key head (token-major), so that all of them share the keys.  An item is as many UNITS as it has blocks of
-// kUnitKeys visible keys, at least one.  All items' units are laid end to end (requests, then tiles, then heads) and every
-// CTA of the grid takes an equal, contiguous stretch: whatever the lengths, the CTAs finish together, and nothing but the
-// lengths on the device decides it (a captured launch replays with new lengths).  A stretch boundary inside an item
-// splits it; each part leaves its unnormalised sum, its maximum and its weight in the workspace, and the CTA that arrives
+// UNIT visible keys, at least one, and weighs COST units more, for what its beginning and end take.  All items are laid end
+// to end (requests, then tiles, then heads) and every CTA of the grid takes an equal, contiguous stretch of that weight:
+// whatever the lengths, the CTAs finish together, and nothing but the lengths on the device decides it (a captured launch
+// replays with new lengths).  A stretch boundary inside an item's units splits it (one inside its COST moves to its
+// beginning); each part leaves its unnormalised sum, its maximum and its weight in the workspace, and the CTA that arrives
 // last (a counter in the workspace) joins them in the order of the keys -- so results do not depend on who was last.
 #pragma once
 #include <cuda_runtime.h>
@@ -61,156 +62,201 @@ template <int TILE, int UNIT>
 __device__ __forceinline__ int paged_tile_units(const PagedParams& p, const PagedRequest& q, int t) {
     return max(1, (paged_tile_end<TILE>(p, q, t) + UNIT - 1) / UNIT);
 }
-// Units of a request for ONE key head.
+constexpr int PAGED_COST = 2;       // measured: an item's end takes about as long as two units' copies
+// Weight of a request's items of ONE key head.
 template <int TILE, int UNIT>
-__device__ __forceinline__ long long paged_request_units(const PagedParams& p, const PagedRequest& q) {
+__device__ __forceinline__ long long paged_request_weight(const PagedParams& p, const PagedRequest& q) {
     long long n = 0;
-    for (int t = 0; t * TILE < q.rows; ++t) n += paged_tile_units<TILE, UNIT>(p, q, t);
+    for (int t = 0; t * TILE < q.rows; ++t) n += paged_tile_units<TILE, UNIT>(p, q, t) + PAGED_COST;
     return n;
 }
 
-// Where a CTA stands in the sequence of items; all threads of the CTA hold the same values.
+// How the launch's weight is shared out: the same for every thread of a CTA, kept in shared memory.
+struct PagedShares {
+    long long lo, total, share;     // this CTA's first position; all weight; weight per CTA (one more for the first `extra` CTAs)
+    int ctas, extra;                // CTAs that have a stretch (never more than weight, so none is empty)
+    int found_r, found_at;          // request of the first position, and its beginning relative to lo
+    long long sums[32];
+};
+// Where a warp stands in the sequence of items.  Positions count from the CTA's first.
 struct PagedCursor {
-    long long lo, hi;               // this CTA's stretch of units
-    long long item;                 // first unit of the current item
-    long long total;                // units of the launch
-    int ctas;                       // CTAs that have a stretch (never more than units, so none is empty)
+    int hi;                         // end of the CTA's stretch
+    int item;                       // beginning of the current item (below 0 where another CTA has it)
     int r, t, h, units;             // current item and its number of units
     PagedRequest q;
+    __device__ __forceinline__ int from() const { return max(0, -item - PAGED_COST); }      // the CTA's part of the item's units
+    __device__ __forceinline__ int to() const { return min(units, hi - item - PAGED_COST); }
+    __device__ __forceinline__ bool more() const { return item + units + 2 * PAGED_COST < hi; }   // of the next item too
 };
 
-// Sums all requests' units (every CTA for itself: 12 bytes per request out of L2) and finds the item where the CTA's
-// stretch begins.  False when the CTA has nothing to do.  `min_units`: no CTA gets fewer, so that short work is not cut
+// Sums all requests' weights (every CTA for itself: 12 bytes per request out of L2) and finds the item where the CTA's
+// stretch begins.  False when the CTA has nothing to do.  `least`: no CTA gets less weight, so that short work is not cut
 // into pieces that cost more to join than to compute.
 template <int THREADS, int TILE, int UNIT>
-__device__ __forceinline__ bool paged_begin(const PagedParams& p, PagedCursor& c, long long* scratch, int min_units) {
+__device__ __forceinline__ bool paged_begin(const PagedParams& p, PagedCursor& c, PagedShares& sh, int least) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int per = (p.requests + THREADS - 1) / THREADS;
     const int r0 = min(static_cast<int>(threadIdx.x) * per, p.requests), r1 = min(r0 + per, p.requests);
     long long mine = 0;
-    for (int r = r0; r < r1; ++r) mine += paged_request_units<TILE, UNIT>(p, paged_request(p, r));
+    for (int r = r0; r < r1; ++r) mine += paged_request_weight<TILE, UNIT>(p, paged_request(p, r));
     mine *= p.kv_heads;
     long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += x; }
-    if (lane == 31) scratch[w] = upto;
+    if (lane == 31) sh.sums[w] = upto;
     __syncthreads();
     long long before = 0, total = 0;
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) { const long long x = scratch[i]; total += x; if (i < w) before += x; }
+    for (int i = 0; i < THREADS / 32; ++i) { const long long x = sh.sums[i]; total += x; if (i < w) before += x; }
     upto += before;
-    c.total = total;
     if (total == 0) return false;
-    c.ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + min_units - 1) / min_units));
-    if (static_cast<int>(blockIdx.x) >= c.ctas) return false;
-    c.lo = total * blockIdx.x / c.ctas;
-    c.hi = total * (blockIdx.x + 1) / c.ctas;
-    __syncthreads();
-    if (upto - mine <= c.lo && c.lo < upto) {
+    const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + least - 1) / least));
+    if (static_cast<int>(blockIdx.x) >= ctas) return false;
+    const long long share = total / ctas;
+    const int extra = static_cast<int>(total - share * ctas);
+    const long long lo = share * blockIdx.x + min(static_cast<int>(blockIdx.x), extra);
+    c.hi = static_cast<int>(share) + (static_cast<int>(blockIdx.x) < extra ? 1 : 0);
+    if (upto - mine <= lo && lo < upto) {
         long long at = upto - mine;
         int r = r0;
         for (;; ++r) {
-            const long long n = paged_request_units<TILE, UNIT>(p, paged_request(p, r)) * p.kv_heads;
-            if (c.lo < at + n) break;
+            const long long n = paged_request_weight<TILE, UNIT>(p, paged_request(p, r)) * p.kv_heads;
+            if (lo < at + n) break;
             at += n;
         }
-        scratch[0] = at; scratch[1] = r;
+        sh.lo = lo; sh.total = total; sh.share = share; sh.ctas = ctas; sh.extra = extra;
+        sh.found_r = r; sh.found_at = static_cast<int>(at - lo);
     }
     __syncthreads();
-    long long at = scratch[0];
-    c.r = static_cast<int>(scratch[1]);
+    int at = sh.found_at;
+    c.r = sh.found_r;
     c.q = paged_request(p, c.r);
     for (c.t = 0;; ++c.t) {
         c.units = paged_tile_units<TILE, UNIT>(p, c.q, c.t);
-        if (c.lo < at + static_cast<long long>(c.units) * p.kv_heads) break;
-        at += static_cast<long long>(c.units) * p.kv_heads;
+        if (at + (c.units + PAGED_COST) * p.kv_heads > 0) break;
+        at += (c.units + PAGED_COST) * p.kv_heads;
     }
-    c.h = static_cast<int>((c.lo - at) / c.units);
-    c.item = at + static_cast<long long>(c.h) * c.units;
-    return true;
+    c.h = -at / (c.units + PAGED_COST);
+    c.item = at + c.h * (c.units + PAGED_COST);
+    return c.to() > 0;
 }
-// To the next item; the caller has checked that there is one (c.item + c.units < c.total).
+// To the next item; the caller has checked that there is one (c.more()).
 template <int TILE, int UNIT>
 __device__ __forceinline__ void paged_next(const PagedParams& p, PagedCursor& c) {
-    c.item += c.units;
+    c.item += c.units + PAGED_COST;
     if (++c.h < p.kv_heads) return;
     c.h = 0;
     ++c.t;
     while (c.t * TILE >= c.q.rows) { c.t = 0; ++c.r; c.q = paged_request(p, c.r); }
     c.units = paged_tile_units<TILE, UNIT>(p, c.q, c.t);
 }
-// CTA whose stretch holds unit u.
-__device__ __forceinline__ int paged_cta_of(const PagedCursor& c, long long u) { return static_cast<int>(((u + 1) * c.ctas - 1) / c.total); }
+// CTA whose stretch holds position u (of the launch).
+__device__ __forceinline__ int paged_cta_of(const PagedShares& s, long long u) {
+    const long long big = (s.share + 1) * s.extra;                 // of the CTAs that have one more
+    return u < big ? static_cast<int>(u / (s.share + 1)) : s.extra + static_cast<int>((u - big) / s.share);
+}
+
+// CTAs with the item's first and last unit.
+__device__ __forceinline__ int paged_first(const PagedShares& s, const PagedCursor& c) { return paged_cta_of(s, s.lo + c.item + PAGED_COST); }
+__device__ __forceinline__ int paged_last(const PagedShares& s, const PagedCursor& c) { return paged_cta_of(s, s.lo + c.item + PAGED_COST + c.units - 1); }
 
 __device__ __forceinline__ float paged_clamp_scale(float s) { return fminf(fmaxf(s, 0x1p-40f), 0x1p72f); }
 
 __device__ __forceinline__ void paged_store2(__nv_bfloat16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
 __device__ __forceinline__ void paged_store2(__half* p, float a, float b) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b); }
 
-// Result of row `row` of the item from its sum `o` (values d, d + 1), weight `l` and reference maximum `m` (log2 units).
-template <typename T, int D>
-__device__ __forceinline__ void paged_finish2(const PagedParams& p, const PagedCursor& c, int row, int d, float o0, float o1, float m, float l) {
+// Result of row `row` of the item from its sums `o` (values d .. d + N - 1), weight `l` and reference maximum `m` (log2 units).
+template <typename T, int D, int N>
+__device__ __forceinline__ void paged_finish(const PagedParams& p, const PagedCursor& c, int row, int d, const float (&o)[N], float m, float l) {
     const int token = row / p.group, head = c.h * p.group + (row - token * p.group);
     const size_t at = static_cast<size_t>(c.q.start) + token;
     const bool none = l == 0.0f;                                   // no key seen: zero and -inf
     const float inv = none ? 0.0f : 1.0f / l;
-    paged_store2(static_cast<T*>(p.out) + at * p.out_stride + static_cast<size_t>(head) * D + d, none ? 0.0f : o0 * inv, none ? 0.0f : o1 * inv);
+    T* dst = static_cast<T*>(p.out) + at * p.out_stride + static_cast<size_t>(head) * D + d;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) paged_store2(dst + i, none ? 0.0f : o[i] * inv, none ? 0.0f : o[i + 1] * inv);
     if (p.lse && d == 0) p.lse[at * (static_cast<size_t>(p.group) * p.kv_heads) + head] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
-// A part of a split item has left its sums in this CTA's partial slot: announce it and, when all parts are there, join them.
-// `rows` rows from tile row 0; scratch: at least (parts + 1) * rows * 2 floats of shared memory.  Called by all threads.
+// The parts of split items that this CTA computed (at most two: the item that its stretch begins in and the one that it
+// ends in) have left their sums in its slots.  At the end of its stretch it announces them and joins the items of which all
+// parts are there now.  Announcing late costs nothing -- somebody has to be last -- and keeps the fence and the round trip
+// of the counters out of the way of the copies.  scratch: 2 (TILE + parts * TILE) floats of shared memory, flags: 2 ints.
 template <typename T, int D, int THREADS, int TILE>
-__device__ __forceinline__ void paged_join(const PagedParams& p, const PagedCursor& c, int rows, int row0, float* scratch, int* flag) {
-    const int first = paged_cta_of(c, c.item), last = paged_cta_of(c, c.item + c.units - 1);
-    const int parts = last - first + 1;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const int before = atomicAdd(p.counters + first, 1);
-        *flag = before == parts - 1;
-        if (before == parts - 1) p.counters[first] = 0;            // as the next call finds it
-    }
-    __syncthreads();
-    if (!*flag) return;
-    __threadfence();
+__device__ __forceinline__ void paged_join(const PagedParams& p, const PagedShares& sh, const PagedCursor& c, float* scratch) {
+    const int first = paged_first(sh, c), parts = paged_last(sh, c) - first + 1;
+    const int row0 = c.t * TILE, rows = min(TILE, c.q.rows - row0);
     constexpr size_t SLOT = static_cast<size_t>(TILE) * (D + 2);
     auto slot = [&](int i) { return p.partials + (static_cast<size_t>(first + i) * 2 + (i == 0 ? 1 : 0)) * SLOT; };
-    // factors of every part for every row: f[i][row] = 2^(m_i - m); the row's m and 1 / weight
-    float* f = scratch;
-    float* ml = scratch + static_cast<size_t>(parts) * rows;
-    for (int i = threadIdx.x; i < parts * rows; i += THREADS) f[i] = __ldcg(slot(i / rows) + TILE * D + i % rows);
+    float* row_m = scratch;                                        // [TILE] maximum, [TILE] weight, [parts][rows] maxima, then factors, [parts][rows] weights
+    float* row_l = scratch + TILE;
+    float* f = scratch + 2 * TILE;
+    float* wl = f + parts * rows;
+    for (int e = threadIdx.x; e < parts * rows; e += THREADS) {
+        const float* ml = slot(e / rows) + TILE * D + e % rows;
+        f[e] = __ldcg(ml); wl[e] = __ldcg(ml + TILE);
+    }
     __syncthreads();
+    const int lane = threadIdx.x & 31;
     for (int row = threadIdx.x >> 5; row < rows; row += THREADS / 32) {      // one warp per row
-        const int lane = threadIdx.x & 31;
-        float m = -INFINITY;
+        float m = -INFINITY, l = 0.0f;
         for (int i = lane; i < parts; i += 32) m = fmaxf(m, f[i * rows + row]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         const float ref = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f;
         for (int i = lane; i < parts; i += 32) {
             const float e = ex2_approx(f[i * rows + row] - ref);
             f[i * rows + row] = e;
-            l += e * __ldcg(slot(i) + TILE * (D + 1) + row);
+            l = fmaf(wl[i * rows + row], e, l);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (lane == 0) { ml[2 * row] = ref; ml[2 * row + 1] = l; }
+        if (lane == 0) { row_m[row] = ref; row_l[row] = l; }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < rows * (D / 2); e += THREADS) {
-        const int row = e / (D / 2), d = (e % (D / 2)) * 2;
-        float o0 = 0.0f, o1 = 0.0f;
-#pragma unroll 4
-        for (int i = 0; i < parts; ++i) {
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(slot(i) + row * D + d));
-            const float w = f[i * rows + row];
-            o0 = fmaf(v.x, w, o0); o1 = fmaf(v.y, w, o1);
+    // the sums: four values per thread and step, sixteen loads in flight
+    for (int e = threadIdx.x; e < rows * (D / 4); e += THREADS) {
+        const int row = e / (D / 4), d = (e % (D / 4)) * 4;
+        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+        for (int i = 0; i < parts; i += 16) {
+            float4 v[16];
+#pragma unroll
+            for (int y = 0; y < 16; ++y) v[y] = i + y < parts ? __ldcg(reinterpret_cast<const float4*>(slot(i + y) + row * D + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int y = 0; y < 16; ++y) {
+                const float w = i + y < parts ? f[(i + y) * rows + row] : 0.0f;
+                o[0] = fmaf(v[y].x, w, o[0]); o[1] = fmaf(v[y].y, w, o[1]); o[2] = fmaf(v[y].z, w, o[2]); o[3] = fmaf(v[y].w, w, o[3]);
+            }
         }
-        paged_finish2<T, D>(p, c, row0 + row, d, o0, o1, ml[2 * row], ml[2 * row + 1]);
+        paged_finish<T, D>(p, c, row0 + row, d, o, row_m[row], row_l[row]);
+    }
+    __syncthreads();                                               // scratch is free again
+}
+
+template <typename T, int D, int THREADS, int TILE>
+__device__ __forceinline__ void paged_announce(const PagedParams& p, const PagedShares& sh, const PagedCursor (&split)[2], const int (&is_split)[2], int* flags, float* scratch) {
+    __syncthreads();                                               // all sums are written, is_split and split are set
+    if (!is_split[0] && !is_split[1]) return;
+    if (threadIdx.x == 0) {
+        __threadfence();                                           // the sums before the arrivals
+        int first[2], parts[2], before[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            flags[i] = 0;
+            if (!is_split[i]) continue;
+            first[i] = paged_first(sh, split[i]);
+            parts[i] = paged_last(sh, split[i]) - first[i] + 1;
+            before[i] = atomicAdd(p.counters + first[i], 1);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (is_split[i] && before[i] == parts[i] - 1) { flags[i] = 1; p.counters[first[i]] = 0; }   // as the next call finds it
+        __threadfence();                                           // the other parts' sums after their arrivals
     }
     __syncthreads();
+    for (int i = 0; i < 2; ++i)
+        if (flags[i]) paged_join<T, D, THREADS, TILE>(p, sh, split[i], scratch);
 }
 
 }  // namespace b200
