@@ -139,7 +139,7 @@ paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         if (w == 0) is_split[0] = is_split[1] = 0;
     }
     PagedCursor c;
-    const bool busy = paged_begin<THREADS, TILE, UNIT>(p, c, shares, 1);
+    const bool busy = paged_begin<THREADS, TILE, UNIT>(p, c, shares);
     __syncthreads();
     if (!busy) return;
     bool ok = true;
@@ -273,11 +273,10 @@ paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         describe();
 #pragma unroll 1
         for (int i = 0; i < S && j0 + i < j1; ++i) note(j0 + i, stage(i));
-        const bool more = c.more();
+        PagedCursor then = c;
+        const bool more = paged_next<TILE, UNIT>(p, then);
         ahead = -1;
         if (more) {                          // what the next item begins with
-            PagedCursor then = c;
-            paged_next<TILE, UNIT>(p, then);
             ahead = block_of(then, 0, then.to(), paged_tile_end<TILE>(p, then.q, then.t));
             load_q(then);
         }

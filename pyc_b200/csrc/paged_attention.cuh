@@ -7,7 +7,7 @@
 // to end (requests, then tiles, then heads) and every CTA of the grid takes an equal, contiguous stretch of that weight:
 // whatever the lengths, the CTAs finish together, and nothing but the lengths on the device decides it (a captured launch
 // replays with new lengths).  A stretch boundary inside an item's units splits it (one inside its COST moves to its
-// beginning); each part leaves its unnormalised sum, its maximum and its weight in the workspace, and the CTA that arrives
+// beginning); short items are never split (a join costs 4 us, eight units 3).  Each part leaves its unnormalised sum, its maximum and its weight in the workspace, and the CTA that arrives
 // last (a counter in the workspace) joins them in the order of the keys -- so results do not depend on who was last.
 #pragma once
 #include <cuda_runtime.h>
@@ -62,6 +62,7 @@ template <int TILE, int UNIT>
 __device__ __forceinline__ int paged_tile_units(const PagedParams& p, const PagedRequest& q, int t) {
     return max(1, (paged_tile_end<TILE>(p, q, t) + UNIT - 1) / UNIT);
 }
+constexpr int PAGED_UNSPLIT = 8;    // items of up to so many units stay whole where the launch has none larger
 constexpr int PAGED_COST = 2;       // measured: an item's end takes about as long as two units' copies
 // Weight of a request's items of ONE key head.
 template <int TILE, int UNIT>
@@ -77,40 +78,48 @@ struct PagedShares {
     int ctas, extra;                // CTAs that have a stretch (never more than weight, so none is empty)
     int found_r, found_at;          // request of the first position, and its beginning relative to lo
     long long sums[32];
+    int most[32];
 };
 // Where a warp stands in the sequence of items.  Positions count from the CTA's first.
 struct PagedCursor {
     int hi;                         // end of the CTA's stretch
     int item;                       // beginning of the current item (below 0 where another CTA has it)
     int r, t, h, units;             // current item and its number of units
+    bool whole;                     // items are not split: one belongs to the CTA with its last position
     PagedRequest q;
-    __device__ __forceinline__ int from() const { return max(0, -item - PAGED_COST); }      // the CTA's part of the item's units
-    __device__ __forceinline__ int to() const { return min(units, hi - item - PAGED_COST); }
-    __device__ __forceinline__ bool more() const { return item + units + 2 * PAGED_COST < hi; }   // of the next item too
+    // the CTA's part of the item's units
+    __device__ __forceinline__ int from() const { return whole ? 0 : max(0, -item - PAGED_COST); }
+    __device__ __forceinline__ int to() const { return whole ? (item + PAGED_COST + units <= hi ? units : 0) : min(units, hi - item - PAGED_COST); }
 };
 
 // Sums all requests' weights (every CTA for itself: 12 bytes per request out of L2) and finds the item where the CTA's
-// stretch begins.  False when the CTA has nothing to do.  `least`: no CTA gets less weight, so that short work is not cut
-// into pieces that cost more to join than to compute.
+// stretch begins.  False when the CTA has nothing to do.
 template <int THREADS, int TILE, int UNIT>
-__device__ __forceinline__ bool paged_begin(const PagedParams& p, PagedCursor& c, PagedShares& sh, int least) {
+__device__ __forceinline__ bool paged_begin(const PagedParams& p, PagedCursor& c, PagedShares& sh) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int per = (p.requests + THREADS - 1) / THREADS;
     const int r0 = min(static_cast<int>(threadIdx.x) * per, p.requests), r1 = min(r0 + per, p.requests);
     long long mine = 0;
-    for (int r = r0; r < r1; ++r) mine += paged_request_weight<TILE, UNIT>(p, paged_request(p, r));
+    int most = 0;
+    for (int r = r0; r < r1; ++r) {
+        const PagedRequest q = paged_request(p, r);
+        mine += paged_request_weight<TILE, UNIT>(p, q);
+        if (q.rows > 0) most = max(most, (q.len + UNIT - 1) / UNIT);
+    }
     mine *= p.kv_heads;
     long long upto = mine;
+    most = __reduce_max_sync(0xffffffffu, most);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += x; }
-    if (lane == 31) sh.sums[w] = upto;
+    if (lane == 31) { sh.sums[w] = upto; sh.most[w] = most; }
     __syncthreads();
     long long before = 0, total = 0;
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) { const long long x = sh.sums[i]; total += x; if (i < w) before += x; }
+    for (int i = 0; i < THREADS / 32; ++i) { const long long x = sh.sums[i]; total += x; if (i < w) before += x; most = max(most, sh.most[i]); }
+    c.whole = most <= PAGED_UNSPLIT;
     upto += before;
     if (total == 0) return false;
-    const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + least - 1) / least));
+    const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
     if (static_cast<int>(blockIdx.x) >= ctas) return false;
     const long long share = total / ctas;
     const int extra = static_cast<int>(total - share * ctas);
@@ -140,15 +149,22 @@ __device__ __forceinline__ bool paged_begin(const PagedParams& p, PagedCursor& c
     c.item = at + c.h * (c.units + PAGED_COST);
     return c.to() > 0;
 }
-// To the next item; the caller has checked that there is one (c.more()).
+// To the CTA's next item; false, and the cursor as it was, when its stretch has no part of it.
 template <int TILE, int UNIT>
-__device__ __forceinline__ void paged_next(const PagedParams& p, PagedCursor& c) {
-    c.item += c.units + PAGED_COST;
-    if (++c.h < p.kv_heads) return;
-    c.h = 0;
-    ++c.t;
-    while (c.t * TILE >= c.q.rows) { c.t = 0; ++c.r; c.q = paged_request(p, c.r); }
-    c.units = paged_tile_units<TILE, UNIT>(p, c.q, c.t);
+__device__ __forceinline__ bool paged_next(const PagedParams& p, PagedCursor& c) {
+    const int item = c.item + c.units + PAGED_COST;
+    if (item + PAGED_COST >= c.hi) return false;                   // also where there is no further request
+    PagedCursor n = c;
+    n.item = item;
+    if (++n.h == p.kv_heads) {
+        n.h = 0;
+        ++n.t;
+        while (n.t * TILE >= n.q.rows) { n.t = 0; ++n.r; n.q = paged_request(p, n.r); }
+        n.units = paged_tile_units<TILE, UNIT>(p, n.q, n.t);
+    }
+    if (n.to() <= 0) return false;
+    c = n;
+    return true;
 }
 // CTA whose stretch holds position u (of the launch).
 __device__ __forceinline__ int paged_cta_of(const PagedShares& s, long long u) {
