@@ -1,8 +1,21 @@
 // Log probabilities of given tokens, entropy and the top alternatives from rows of logits, and the gradient
 // (formulas and meaning: include/pyc_b200.h).  PyC has no counterpart; the row softmax is in elementwise.cu.
 //
-// One CTA per row.  The statistics take one pass with a running maximum m, s = sum e^(x - m) and t = sum (x - m) e^(x - m)
-// (lse = m + ln s, entropy = ln s - t / s); each alternative takes another pass for the largest logit behind the previous one.
+// Forward: one pass over the row.  Each thread keeps a running maximum m, s = sum e^(x - m) and t = sum (x - m) e^(x - m);
+// joined, lse = m + ln s and entropy = ln s - t / s.  Bound by reading the logits: 16-byte loads, four in flight per thread,
+// and five issue slots per element (packed clamp and maximum on 16-bit pairs, packed f32 arithmetic, one exponential).
+//
+// The alternatives come out of the same pass.  The k-th largest of the THREADS threads' maxima, tau, is a lower bound of the k-th
+// largest logit (k distinct elements reach it), and only threads whose maximum reaches tau can hold one: a handful of
+// threads' elements are read again (they are in L2) and what exceeds tau is ranked.  tau is found by a bisection over the
+// ordered bits with block-wide counts.  Many ties at tau (coarse logits, a vocabulary masked down to a few tokens) end in a scan of the
+// row from its start, which is where the ties that count are; see top_of_slice.
+//
+// Rows are taken by one CTA each; where there are fewer rows than the SMs can hold, a cluster of 2, 4 or 8 CTAs shares a row
+// and its first CTA joins the others' statistics and candidates through distributed shared memory.
+//
+// -inf is clamped to the type's lowest value on the way in, so that nothing multiplies 0 by infinity; a row whose maximum is
+// that lowest value (all masked) is done again exactly.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -14,109 +27,479 @@ namespace {
 
 constexpr int LT = 256;
 constexpr int MAX_TOP = 32;
+constexpr int MAX_CAND = 1024;
+constexpr float LOG2E = 1.4426950408889634f;
 
-__device__ __forceinline__ float logit(const float* x, size_t i) { return x[i]; }
-__device__ __forceinline__ float logit(const __nv_bfloat16* x, size_t i) { return __bfloat162float(x[i]); }
-__device__ __forceinline__ float logit(const __half* x, size_t i) { return __half2float(x[i]); }
-__device__ __forceinline__ void put(float* x, size_t i, float v) { x[i] = v; }
-__device__ __forceinline__ void put(__nv_bfloat16* x, size_t i, float v) { x[i] = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void put(__half* x, size_t i, float v) { x[i] = __float2half_rn(v); }
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// Per type: 16-byte vectors of N elements as f32, clamped to the type's lowest value (NaN stays), with their maximum.
+template <typename T> struct Logits;
+template <> struct Logits<float> {
+    static constexpr int N = 4, F32_BITS = 32;
+    static __device__ __forceinline__ float lowest() { return -3.4028234663852886e38f; }
+    static __device__ __forceinline__ float one(const float* p) { return *p; }
+    static __device__ __forceinline__ void store(float* p, float v) { *p = v; }
+    static __device__ __forceinline__ float unpack(const uint4& u, float (&f)[4]) {
+        f[0] = max_nan(__uint_as_float(u.x), lowest()); f[1] = max_nan(__uint_as_float(u.y), lowest());
+        f[2] = max_nan(__uint_as_float(u.z), lowest()); f[3] = max_nan(__uint_as_float(u.w), lowest());
+        return max_nan(max_nan(f[0], f[1]), max_nan(f[2], f[3]));
+    }
+    static __device__ __forceinline__ void raw(const uint4& u, float (&f)[4]) {
+        f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[4]) { return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])); }
+};
+template <> struct Logits<__nv_bfloat16> {
+    static constexpr int N = 8, F32_BITS = 16;
+    static __device__ __forceinline__ float lowest() { return -3.3895313892515355e38f; }
+    static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+    static __device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { uint32_t d; asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b)); return d; }
+    static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
+    static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+    static __device__ __forceinline__ float unpack(const uint4& u, float (&f)[8]) {
+        constexpr uint32_t LOW = 0xff7fff7fu;
+        const uint32_t a = max2(u.x, LOW), b = max2(u.y, LOW), c = max2(u.z, LOW), d = max2(u.w, LOW), m = max2(max2(a, b), max2(c, d));
+        f[0] = lo(a); f[1] = hi(a); f[2] = lo(b); f[3] = hi(b); f[4] = lo(c); f[5] = hi(c); f[6] = lo(d); f[7] = hi(d);
+        return max_nan(lo(m), hi(m));
+    }
+    static __device__ __forceinline__ void raw(const uint4& u, float (&f)[8]) {
+        f[0] = lo(u.x); f[1] = hi(u.x); f[2] = lo(u.y); f[3] = hi(u.y); f[4] = lo(u.z); f[5] = hi(u.z); f[6] = lo(u.w); f[7] = hi(u.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t*>(&h); }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <> struct Logits<__half> {
+    static constexpr int N = 8, F32_BITS = 19;
+    static __device__ __forceinline__ float lowest() { return -65504.0f; }
+    static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
+    static __device__ __forceinline__ void store(__half* p, float v) { *p = __float2half_rn(v); }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { uint32_t d; asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b)); return d; }
+    static __device__ __forceinline__ float2 both(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+    static __device__ __forceinline__ void split(uint32_t a, uint32_t b, uint32_t c, uint32_t d, float (&f)[8]) {
+        const float2 p = both(a), q = both(b), r = both(c), s = both(d);
+        f[0] = p.x; f[1] = p.y; f[2] = q.x; f[3] = q.y; f[4] = r.x; f[5] = r.y; f[6] = s.x; f[7] = s.y;
+    }
+    static __device__ __forceinline__ float unpack(const uint4& u, float (&f)[8]) {
+        constexpr uint32_t LOW = 0xfbfffbffu;
+        const uint32_t a = max2(u.x, LOW), b = max2(u.y, LOW), c = max2(u.z, LOW), d = max2(u.w, LOW);
+        split(a, b, c, d, f);
+        const float2 m = both(max2(max2(a, b), max2(c, d)));
+        return max_nan(m.x, m.y);
+    }
+    static __device__ __forceinline__ void raw(const uint4& u, float (&f)[8]) { split(u.x, u.y, u.z, u.w, f); }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t*>(&h); }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
 
 struct Stats { float m, s, t; };
-// Joins two running sums; a side that has seen nothing (m = -inf) contributes nothing.
+// Joins two running sums.  A side whose factor has vanished contributes nothing, however large its distance (0 * inf).
 __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
     Stats c;
     c.m = fmaxf(a.m, b.m);
     const float da = a.m == c.m ? 0.0f : a.m - c.m, db = b.m == c.m ? 0.0f : b.m - c.m;
-    const float ea = expf(da), eb = expf(db);
+    const float ea = ex2_approx(da * LOG2E), eb = ex2_approx(db * LOG2E);
     c.s = a.s * ea + b.s * eb;
-    // a side whose factor has vanished contributes nothing, however large its distance (0 * inf)
     c.t = (a.s * ea > 0.0f ? (a.t + a.s * da) * ea : 0.0f) + (b.s * eb > 0.0f ? (b.t + b.s * db) * eb : 0.0f);
     return c;
 }
+__device__ __forceinline__ Stats warp_join(Stats a) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        Stats b;
+        b.m = __shfl_xor_sync(0xffffffffu, a.m, o); b.s = __shfl_xor_sync(0xffffffffu, a.s, o); b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
+        a = join(a, b);
+    }
+    return a;
+}
 
+// Values ordered as unsigned numbers (minus zero with plus zero), and back.
+__device__ __forceinline__ uint32_t ordered(float v) { const uint32_t u = __float_as_uint(v + 0.0f); return u & 0x80000000u ? ~u : u | 0x80000000u; }
+__device__ __forceinline__ float from_ordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+// Larger value first, then the lower index: one number, never 0.
+__device__ __forceinline__ unsigned long long key_of(float v, uint32_t index) { return (static_cast<unsigned long long>(ordered(v)) << 32) | (0xffffffffu - index); }
+
+// The part of a row that a CTA reads: single elements up to the first 16-byte boundary (first CTA), vectors, single elements.
+struct Slice { uint32_t head, tail, tail0, v0, v1, base; };      // vectors [v0, v1), vector v holds elements base + v * N ..
+
+struct Shared {
+    Stats warp[LT / 32], all;
+    unsigned long long cand[MAX_CAND];
+    unsigned long long top[MAX_TOP];       // the slice's, sorted; 0: none
+    uint32_t who[LT];
+    uint32_t gt_threads, gt, eq, scan[LT / 32];
+    int bad;
+};
+
+// All elements of thread `who`'s share, in no order: f(value, index).  Called by one warp.
+template <typename T, typename F>
+__device__ __forceinline__ void share_of(const T* x, const Slice& sl, uint32_t who, const F& f) {
+    constexpr int N = Logits<T>::N;
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t v = sl.v0 + who + lane * LT; v < sl.v1; v += 32 * LT) {
+        float e[N];
+        Logits<T>::raw(__ldg(reinterpret_cast<const uint4*>(x + sl.base) + v), e);
+#pragma unroll
+        for (int i = 0; i < N; ++i) f(e[i], sl.base + v * N + i);
+    }
+    if (lane == 0 && who < sl.head) f(Logits<T>::one(x + who), who);
+    if (lane == 1 && who < sl.tail) f(Logits<T>::one(x + sl.tail0 + who), sl.tail0 + who);
+}
+// Element i of the slice in the order of the row.
+__device__ __forceinline__ uint32_t slice_size(const Slice& sl, int n) { return sl.head + (sl.v1 - sl.v0) * n + sl.tail; }
+__device__ __forceinline__ uint32_t slice_at(const Slice& sl, int n, uint32_t i) {
+    if (i < sl.head) return i;
+    i -= sl.head;
+    const uint32_t mid = (sl.v1 - sl.v0) * n;
+    return i < mid ? sl.base + sl.v0 * n + i : sl.tail0 + (i - mid);
+}
+
+// The slice's k largest by (value, lower index) into sh.top.  `tmax`: the thread's maximum of its clamped elements.
 template <typename T>
-__global__ void __launch_bounds__(LT)
-token_logprobs_kernel(pyc_b200_token_logprobs_args p) {
-    __shared__ Stats st[LT];
-    __shared__ unsigned long long best[LT];
-    __shared__ int broken;
-    const size_t row = blockIdx.x;
-    const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
-    if (threadIdx.x == 0) broken = 0;
+__device__ void top_of_slice(const T* x, const Slice& sl, int k, float tmax, bool any, Shared& sh) {
+    constexpr int N = Logits<T>::N;
+    const float low = Logits<T>::lowest();
+    if (threadIdx.x < MAX_TOP) sh.top[threadIdx.x] = 0;
+    if (threadIdx.x == 0) { sh.gt_threads = 0; sh.gt = 0; sh.eq = 0; }
+    // tau: the largest value that k threads' maxima reach; below every value when fewer than k threads have elements
+    const uint32_t mine = any ? ordered(tmax) : 0;
+    uint32_t tau = 0;
+    // the bits of f32 that the type fills; those below are all 0 (positive) or, ordered, all 1 (negative) and follow from the sign
+    constexpr int BITS = Logits<T>::F32_BITS;
+#pragma unroll 1
+    for (int b = 31; b >= 32 - BITS; --b) {
+        const uint32_t trial = tau | (1u << b);
+        if (__syncthreads_count(mine >= trial) >= k) tau = trial;
+    }
+    if (BITS < 32 && tau != 0 && !(tau & 0x80000000u)) tau |= static_cast<uint32_t>((1ull << (32 - BITS)) - 1);
+    const bool few = tau == 0;
+    const float tau_v = from_ordered(tau);
+    const bool masked = !few && tau_v <= low;             // the class of -inf and the lowest value: told apart below
+    if (any && (few || mine > tau)) sh.who[atomicAdd(&sh.gt_threads, 1)] = threadIdx.x;
+    if (any && !few && mine == tau) { const uint32_t e = atomicAdd(&sh.eq, 1); if (e < 64) sh.who[LT - 1 - e] = threadIdx.x; }
     __syncthreads();
-    Stats a = {-INFINITY, 0.0f, 0.0f};
-    bool bad = false;
-    for (size_t i = threadIdx.x; i < p.vocab; i += LT) {
-        const float v = logit(x, i);
-        bad |= !(v < INFINITY);
-        if (v == -INFINITY) continue;
-        const Stats one = {v, 1.0f, 0.0f};
-        a = join(a, one);
-    }
-    if (bad) broken = 1;
-    st[threadIdx.x] = a;
+    const uint32_t gt_threads = sh.gt_threads, eq_threads = sh.eq;
+    const bool scan = !few && (masked || eq_threads > 64 || gt_threads + eq_threads > LT);
     __syncthreads();
-    for (int o = LT / 2; o > 0; o >>= 1) {
-        if (threadIdx.x < o) st[threadIdx.x] = join(st[threadIdx.x], st[threadIdx.x + o]);
-        __syncthreads();
+    if (threadIdx.x == 0) sh.eq = 0;
+    __syncthreads();
+    // candidates above tau (few: all), and with few threads at tau those that equal it
+    const uint32_t lists = gt_threads + (scan ? 0 : eq_threads);
+    for (uint32_t i = threadIdx.x >> 5; i < lists; i += LT / 32) {
+        const uint32_t who = i < gt_threads ? sh.who[i] : sh.who[LT - 1 - (i - gt_threads)];
+        share_of<T>(x, sl, who, [&](float v, uint32_t index) {
+            const bool take = few || (scan ? ordered(v) > tau && v > low : ordered(v) >= tau);
+            if (take) { const uint32_t at = atomicAdd(&sh.gt, 1); if (at < MAX_CAND) sh.cand[at] = key_of(v, index); }
+        });
     }
-    const Stats all = st[0];
-    const bool none = all.m == -INFINITY;
-    const float nan = __int_as_float(0x7fffffff);
-    // log probabilities are (x - m) - ln s: x - lse would lose ln s beside a large maximum
-    const float ln_s = logf(all.s), lse = broken ? nan : none ? -INFINITY : all.m + ln_s;
-    if (threadIdx.x == 0) {
-        const int tok = p.tokens[row];
-        const bool given = tok >= 0 && static_cast<size_t>(tok) < p.vocab;
-        p.logprob[row] = broken ? nan : !given ? 0.0f : none ? -INFINITY : (logit(x, tok) - all.m) - ln_s;
-        if (p.lse) p.lse[row] = lse;
-        if (p.entropy) p.entropy[row] = broken ? nan : none ? 0.0f : ln_s - all.t / all.s;
-    }
-    // value, then lower index: one ordered 64-bit key; each round takes the largest key below the last one
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < p.top_k; ++k) {
-        unsigned long long mine = 0;
-        for (size_t i = threadIdx.x; i < p.vocab; i += LT) {
-            const unsigned u = __float_as_uint(logit(x, i) + 0.0f);
-            const unsigned long long key = (static_cast<unsigned long long>(u & 0x80000000u ? ~u : u | 0x80000000u) << 32) | (0xffffffffu - static_cast<unsigned>(i));
-            if (key < last && key > mine) mine = key;
-        }
-        best[threadIdx.x] = mine;
-        __syncthreads();
-        for (int o = LT / 2; o > 0; o >>= 1) {
-            if (threadIdx.x < o && best[threadIdx.x + o] > best[threadIdx.x]) best[threadIdx.x] = best[threadIdx.x + o];
+    __syncthreads();
+    uint32_t n = sh.gt;
+    if (n <= MAX_CAND && scan && n < static_cast<uint32_t>(k)) {
+        // ties at tau: the lowest indices, in order.  masked: first the elements of the lowest value, then -inf; they are kept apart
+        // in the two halves of what is left of the buffer (n < 32 is taken).
+        const uint32_t need = k - n, size = slice_size(sl, N);
+        uint32_t found = 0, found_inf = 0;
+        for (uint32_t i0 = 0; i0 < size && found < need; i0 += LT) {
+            const uint32_t i = i0 + threadIdx.x;
+            const uint32_t index = i < size ? slice_at(sl, N, i) : 0;
+            const float v = i < size ? Logits<T>::one(x + index) : INFINITY;
+            const bool hit = i < size && (masked ? v == low : ordered(v) == tau), inf = masked && v == -INFINITY;
+            const unsigned mh = __ballot_sync(0xffffffffu, hit), mi = __ballot_sync(0xffffffffu, inf);
+            const uint32_t w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+            if (lane == 0) sh.scan[w] = __popc(mh) | (__popc(mi) << 16);
+            __syncthreads();
+            uint32_t before = 0, total = 0;
+#pragma unroll
+            for (uint32_t y = 0; y < LT / 32; ++y) { total += sh.scan[y]; before += y < w ? sh.scan[y] : 0; }
+            const uint32_t at = found + (before & 0xffffu) + __popc(mh & ((1u << lane) - 1u)), ai = found_inf + (before >> 16) + __popc(mi & ((1u << lane) - 1u));
+            if (hit && at < need) sh.cand[n + at] = key_of(v, index);
+            if (inf && ai < need) sh.cand[MAX_CAND / 2 + ai] = key_of(v, index);
+            found += total & 0xffffu; found_inf += total >> 16;
             __syncthreads();
         }
-        last = best[0];
-        if (threadIdx.x == 0) {
-            const unsigned i = 0xffffffffu - static_cast<unsigned>(last);
-            p.top_ids[row * p.top_k + k] = broken ? -1 : static_cast<int>(i);
-            p.top_logprobs[row * p.top_k + k] = broken ? nan : none ? -INFINITY : (logit(x, i) - all.m) - ln_s;
+        found = min(found, need);
+        const uint32_t rest = min(found_inf, need - found);
+        if (threadIdx.x < rest) sh.cand[n + found + threadIdx.x] = sh.cand[MAX_CAND / 2 + threadIdx.x];
+        n += found + rest;
+        __syncthreads();
+    }
+    if (n <= MAX_CAND) {
+        // the rank of a candidate is the number of larger ones; keys are distinct
+        for (uint32_t i = threadIdx.x; i < n; i += LT) {
+            const unsigned long long mine_key = sh.cand[i];
+            uint32_t rank = 0;
+            for (uint32_t y = 0; y < n; ++y) rank += sh.cand[y] > mine_key;
+            if (rank < static_cast<uint32_t>(k)) sh.top[rank] = mine_key;
         }
+        __syncthreads();
+        return;
+    }
+    // more than MAX_CAND elements above tau in the shares of fewer than k threads: one after the other
+    const uint32_t size = slice_size(sl, N);
+    unsigned long long last = ~0ull;
+    for (int r = 0; r < k; ++r) {
+        unsigned long long best = 0;
+        for (uint32_t i = threadIdx.x; i < size; i += LT) {
+            const uint32_t index = slice_at(sl, N, i);
+            const unsigned long long key = key_of(Logits<T>::one(x + index), index);
+            if (key < last && key > best) best = key;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) { const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, o); best = y > best ? y : best; }
+        if ((threadIdx.x & 31) == 0) sh.cand[threadIdx.x >> 5] = best;
+        __syncthreads();
+        for (int y = 0; y < LT / 32; ++y) best = sh.cand[y] > best ? sh.cand[y] : best;
+        if (threadIdx.x == 0) sh.top[r] = best;
+        last = best;
         __syncthreads();
     }
 }
 
+__device__ __forceinline__ uint32_t peer_address(const void* p, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float peer_float(uint32_t a) { float v; asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory"); return v; }
+__device__ __forceinline__ unsigned long long peer_u64(uint32_t a) { unsigned long long v; asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory"); return v; }
+__device__ __forceinline__ void cluster_barrier() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 template <typename T>
 __global__ void __launch_bounds__(LT)
-token_logprobs_grad_kernel(pyc_b200_token_logprobs_grad_args p) {
-    const size_t row = blockIdx.x;
+token_logprobs_kernel(pyc_b200_token_logprobs_args p, int ctas) {
+    constexpr int N = Logits<T>::N;
+    __shared__ Shared sh;
+    const float low = Logits<T>::lowest();
+    const size_t row = blockIdx.x / ctas;
+    const uint32_t part = blockIdx.x % ctas;              // = the rank in the cluster
+    const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
+    const uint32_t vocab = static_cast<uint32_t>(p.vocab);
+    Slice sl;
+    {
+        const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+        const uint32_t lead = min(off ? N - off : 0u, vocab), nv = (vocab - lead) / N;
+        sl.base = lead;
+        sl.v0 = static_cast<uint32_t>(static_cast<uint64_t>(nv) * part / ctas); sl.v1 = static_cast<uint32_t>(static_cast<uint64_t>(nv) * (part + 1) / ctas);
+        sl.head = part == 0 ? lead : 0;
+        sl.tail0 = lead + nv * N;
+        sl.tail = part + 1 == static_cast<uint32_t>(ctas) ? vocab - sl.tail0 : 0;
+    }
+    if (threadIdx.x == 0) sh.bad = 0;
+
+    // ---- the pass
+    Stats a = {low, 0.0f, 0.0f};
+    bool bad = false;
+    auto raise = [&](float m) {                           // the reference moves up to m
+        const float d = a.m - m, e = ex2_approx(d * LOG2E);
+        a.t = e > 0.0f ? (a.t + a.s * d) * e : 0.0f;
+        a.s *= e;
+        a.m = m;
+    };
+    auto take = [&](float v) {
+        v = max_nan(v, low);
+        bad |= !(v < INFINITY);
+        if (v > a.m) raise(v);
+        const float d = v - a.m, e = ex2_approx(d * LOG2E);
+        a.s += e; a.t = fmaf(e, d, a.t);
+    };
+    if (threadIdx.x < sl.head) take(Logits<T>::one(x + threadIdx.x));
+    if (threadIdx.x < sl.tail) take(Logits<T>::one(x + sl.tail0 + threadIdx.x));
+    const uint4* xv = reinterpret_cast<const uint4*>(x + sl.base);
+    const unsigned long long log2e2 = f32x2_splat(LOG2E);
+    unsigned long long s2 = 0, t2 = 0;                    // packed sums beside a.s, a.t: (0, 0)
+    constexpr int U = 4;
+    for (uint32_t v = sl.v0 + threadIdx.x; v < sl.v1; v += U * LT) {
+        uint4 u[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) u[i] = v + i * LT < sl.v1 ? __ldg(xv + v + i * LT) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (v + i * LT >= sl.v1) break;
+            float f[N];
+            const float m = Logits<T>::unpack(u[i], f);
+            bad |= !(m < INFINITY);
+            if (m > a.m) {
+                float x0, x1;
+                f32x2_unpack(s2, x0, x1); a.s += x0 + x1;
+                f32x2_unpack(t2, x0, x1); a.t += x0 + x1;
+                s2 = t2 = 0;
+                raise(m);
+            }
+            const unsigned long long minus = f32x2_splat(-a.m);
+#pragma unroll
+            for (int y = 0; y < N; y += 2) {
+                const unsigned long long d = f32x2_add(f32x2_pack(f[y], f[y + 1]), minus);
+                float y0, y1;
+                f32x2_unpack(f32x2_mul(d, log2e2), y0, y1);
+                const unsigned long long e = f32x2_pack(ex2_approx(y0), ex2_approx(y1));
+                s2 = f32x2_add(s2, e);
+                t2 = f32x2_fma(e, d, t2);
+            }
+        }
+    }
+    {
+        float x0, x1;
+        f32x2_unpack(s2, x0, x1); a.s += x0 + x1;
+        f32x2_unpack(t2, x0, x1); a.t += x0 + x1;
+    }
+    const bool any = threadIdx.x < sl.head || threadIdx.x < sl.tail || sl.v0 + threadIdx.x < sl.v1;
+    const float tmax = a.m;
+    __syncthreads();                                      // sh.bad is zero
+    if (bad) sh.bad = 1;
+    const Stats w = warp_join(a);
+    if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = w;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        Stats c = sh.warp[0];
+        for (int i = 1; i < LT / 32; ++i) c = join(c, sh.warp[i]);
+        sh.all = c;
+    }
+    const bool slice_bad = sh.bad != 0;
+    if (p.top_k && !slice_bad) top_of_slice<T>(x, sl, p.top_k, tmax, any, sh);
+    __syncthreads();
+
+    // ---- the row: the first CTA joins the others
+    if (ctas > 1) {
+        cluster_barrier();
+        if (part == 0) {
+            if (threadIdx.x == 0) {
+                Stats c = sh.all;
+                int broken = sh.bad;
+                for (int r = 1; r < ctas; ++r) {
+                    const uint32_t at = peer_address(&sh.all, r);
+                    const Stats o = {peer_float(at), peer_float(at + 4), peer_float(at + 8)};
+                    broken |= __float_as_int(peer_float(peer_address(&sh.bad, r)));
+                    c = join(c, o);
+                }
+                sh.all = c;
+                sh.bad = broken;
+            }
+            if (p.top_k) {
+                // up to 8 sorted lists of up to 32 keys: 256 candidates
+                unsigned long long key = 0;
+                const int r = threadIdx.x / MAX_TOP, i = threadIdx.x % MAX_TOP;
+                if (r < ctas) key = r == 0 ? sh.top[i] : peer_u64(peer_address(&sh.top[i], r));
+                __syncthreads();
+                sh.cand[threadIdx.x] = key;
+                __syncthreads();
+                uint32_t rank = 0;
+                for (int y = 0; y < ctas * MAX_TOP; ++y) rank += sh.cand[y] > key;
+                if (key && rank < static_cast<uint32_t>(p.top_k)) sh.top[rank] = key;
+            }
+        }
+        cluster_barrier();                                // nobody leaves while its memory is read
+        if (part != 0) return;
+        __syncthreads();
+    }
+    const bool broken = sh.bad != 0;
+    if (!broken && (sh.all.m <= low || sh.all.m > 1e30f)) {
+        // nothing but masked logits, or ones beside which the clamp would show: the row once more, exactly
+        Stats c = {-INFINITY, 0.0f, 0.0f};
+        for (uint32_t i = threadIdx.x; i < vocab; i += LT) {
+            const float v = Logits<T>::one(x + i);
+            if (v != -INFINITY) c = join(c, Stats{v, 1.0f, 0.0f});
+        }
+        c = warp_join(c);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = c;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            c = sh.warp[0];
+            for (int i = 1; i < LT / 32; ++i) c = join(c, sh.warp[i]);
+            sh.all = c;
+        }
+    }
+    __syncthreads();
+    const Stats all = sh.all;
+    const bool none = all.m == -INFINITY;
+    const float nan = __int_as_float(0x7fffffff);
+    // log probabilities are (x - m) - ln s: x - lse would lose ln s beside a large maximum
+    const float ln_s = logf(all.s);
+    if (threadIdx.x == 0) {
+        const int tok = p.tokens[row];
+        const bool given = tok >= 0 && static_cast<uint32_t>(tok) < vocab;
+        p.logprob[row] = broken ? nan : !given ? 0.0f : none ? -INFINITY : (Logits<T>::one(x + tok) - all.m) - ln_s;
+        if (p.lse) p.lse[row] = broken ? nan : none ? -INFINITY : all.m + ln_s;
+        if (p.entropy) p.entropy[row] = broken ? nan : none ? 0.0f : fmaxf(ln_s - all.t / all.s, 0.0f);
+    }
+    if (static_cast<int>(threadIdx.x) < p.top_k) {
+        const unsigned long long key = sh.top[threadIdx.x];
+        p.top_ids[row * p.top_k + threadIdx.x] = broken ? -1 : static_cast<int>(0xffffffffu - static_cast<uint32_t>(key));
+        p.top_logprobs[row * p.top_k + threadIdx.x] = broken ? nan : none ? -INFINITY : (from_ordered(static_cast<uint32_t>(key >> 32)) - all.m) - ln_s;
+    }
+}
+
+// ---- gradient: reads and writes each element once, bound by that.  One CTA per row and chunk of GRAD_CHUNK vectors; 16-byte
+// accesses where logits and gradient lie equally to a 16-byte boundary, single elements otherwise.
+constexpr int GRAD_U = 4, GRAD_CHUNK = LT * GRAD_U * 2;
+
+template <typename T>
+__global__ void __launch_bounds__(LT)
+token_logprobs_grad_kernel(pyc_b200_token_logprobs_grad_args p, uint32_t chunks) {
+    constexpr int N = Logits<T>::N;
+    const size_t row = blockIdx.x / chunks;
+    const uint32_t chunk = blockIdx.x % chunks, vocab = static_cast<uint32_t>(p.vocab);
     const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
     T* d = static_cast<T*>(p.grad_logits) + row * p.grad_stride;
-    const float lse = p.lse[row];
-    const float u = p.grad_logprob ? p.grad_logprob[row] : 0.0f, w = p.grad_entropy ? p.grad_entropy[row] : 0.0f;
-    const float ent = w != 0.0f ? p.entropy[row] : 0.0f;
-    const int tok = p.tokens[row];
-    const bool given = tok >= 0 && static_cast<size_t>(tok) < p.vocab;
-    const float c = (given ? u : 0.0f) + w * ent;
-    for (size_t i = threadIdx.x; i < p.vocab; i += LT) {
-        const float v = logit(x, i);
-        const float lp = v - lse;
-        float g = 0.0f;
-        if (v != -INFINITY) g = -expf(lp) * (c + w * lp);
-        if (given && i == static_cast<size_t>(tok) && lse != -INFINITY) g += u;
-        put(d, i, g);
+    const float lse = __ldg(p.lse + row);
+    const float u = p.grad_logprob ? __ldg(p.grad_logprob + row) : 0.0f, w = p.grad_entropy ? __ldg(p.grad_entropy + row) : 0.0f;
+    const int tok = __ldg(p.tokens + row);
+    const bool given = tok >= 0 && static_cast<uint32_t>(tok) < vocab;
+    const float c = (given ? u : 0.0f) + (w != 0.0f ? w * __ldg(p.entropy + row) : 0.0f);
+    const bool none = lse == -INFINITY;
+    // -inf logits: log p is held at -1e30, so that p (c + w log p) is 0, not 0 * inf
+    auto grad = [&](float v) {
+        const float lp = max_nan(v - lse, -1e30f);
+        return none ? 0.0f : -ex2_approx(lp * LOG2E) * fmaf(w, lp, c);
+    };
+    auto one = [&](uint32_t i) {
+        float g = grad(Logits<T>::one(x + i));
+        if (given && !none && i == static_cast<uint32_t>(tok)) g += u;
+        Logits<T>::store(d + i, g);
+    };
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)), off_d = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(d) % 16 / sizeof(T));
+    if (off != off_d) {
+        const uint32_t i0 = chunk * (GRAD_CHUNK * N), i1 = min(vocab, i0 + GRAD_CHUNK * N);
+        for (uint32_t i = i0 + threadIdx.x; i < i1; i += LT) one(i);
+        return;
+    }
+    const uint32_t lead = min(off ? N - off : 0u, vocab), nv = (vocab - lead) / N, tail0 = lead + nv * N;
+    if (chunk == 0) {
+        if (threadIdx.x < lead) one(threadIdx.x);
+        if (tail0 + threadIdx.x < vocab && threadIdx.x < N) one(tail0 + threadIdx.x);
+    }
+    const uint4* xv = reinterpret_cast<const uint4*>(x + lead);
+    uint4* dv = reinterpret_cast<uint4*>(d + lead);
+    const uint32_t end = min(nv, (chunk + 1) * GRAD_CHUNK);
+    for (uint32_t v = chunk * GRAD_CHUNK + threadIdx.x; v < end; v += GRAD_U * LT) {
+        uint4 r[GRAD_U];
+#pragma unroll
+        for (int i = 0; i < GRAD_U; ++i) if (v + i * LT < end) r[i] = xv[v + i * LT];
+#pragma unroll
+        for (int i = 0; i < GRAD_U; ++i) {
+            if (v + i * LT >= end) break;
+            float f[N];
+            Logits<T>::raw(r[i], f);
+#pragma unroll
+            for (int y = 0; y < N; ++y) f[y] = grad(f[y]);
+            const uint32_t at = lead + (v + i * LT) * N;
+            if (given && !none && static_cast<uint32_t>(tok) - at < static_cast<uint32_t>(N)) {
+#pragma unroll
+                for (int y = 0; y < N; ++y) if (static_cast<uint32_t>(tok) == at + y) f[y] += u;
+            }
+            dv[v + i * LT] = Logits<T>::pack(f);
+        }
     }
 }
 
@@ -125,6 +508,33 @@ bool logits_ok(pyc_dtype t, size_t rows, size_t vocab, size_t stride) {
     if (rows == 0 || vocab == 0 || rows > 0x7fffffffull || vocab > 0x7fffffffull) { set_error("token logprobs: rows and vocab must be 1 .. 2^31 - 1"); return false; }
     if (stride < vocab) { set_error("token logprobs: row stride %zu below vocab %zu", stride, vocab); return false; }
     return true;
+}
+bool aligned_to(const void* q, pyc_dtype t) { return reinterpret_cast<uintptr_t>(q) % dtype_size(t) == 0; }
+
+template <typename T>
+int launch_scores(const pyc_b200_token_logprobs_args& p, cudaStream_t s) {
+    // CTAs per row: enough for two per SM, while each has some 16-byte vectors per thread
+    int ctas = 1;
+    while (ctas < 8 && p.rows * ctas < static_cast<size_t>(sm_count()) * 2 && p.vocab / (ctas * 2) >= static_cast<size_t>(2 * LT * Logits<T>::N)) ctas *= 2;
+    if (p.rows * ctas > 0x7fffffffull) ctas = 1;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ctas; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(p.rows * ctas)); cfg.blockDim = dim3(LT); cfg.stream = s; cfg.attrs = &attr; cfg.numAttrs = ctas > 1 ? 1 : 0;
+    B200_CUDA_OK(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, p, ctas));
+    count_launch();
+    return 0;
+}
+
+template <typename T>
+int launch_grad(const pyc_b200_token_logprobs_grad_args& p, cudaStream_t s) {
+    const size_t chunks = (p.vocab + static_cast<size_t>(GRAD_CHUNK) * Logits<T>::N - 1) / (static_cast<size_t>(GRAD_CHUNK) * Logits<T>::N);
+    if (p.rows * chunks > 0x7fffffffull) { set_error("token logprobs backward: rows * vocab is too large for one launch"); return -1; }
+    token_logprobs_grad_kernel<T><<<static_cast<unsigned>(p.rows * chunks), LT, 0, s>>>(p, static_cast<uint32_t>(chunks));
+    B200_CUDA_OK(cudaGetLastError());
+    count_launch();
+    return 0;
 }
 
 }  // namespace
@@ -139,16 +549,13 @@ int pyc_b200_token_logprobs(const pyc_b200_token_logprobs_args* a, void* stream)
     pyc_b200_token_logprobs_args p = *a;
     if (!p.row_stride) p.row_stride = p.vocab;
     if (!logits_ok(p.dtype, p.rows, p.vocab, p.row_stride)) return -1;
+    if (!aligned_to(p.logits, p.dtype)) { set_error("token logprobs: logits are not aligned to their type"); return -1; }
     if (p.top_k < 0 || p.top_k > MAX_TOP || static_cast<size_t>(p.top_k) > p.vocab) { set_error("token logprobs: top_k %d is not in 0 .. min(%d, vocab)", p.top_k, MAX_TOP); return -1; }
     if (p.top_k && (!p.top_ids || !p.top_logprobs)) { set_error("token logprobs: top_k without top_ids and top_logprobs"); return -1; }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const unsigned grid = static_cast<unsigned>(p.rows);
-    if (p.dtype == PYC_DTYPE_F32) token_logprobs_kernel<float><<<grid, LT, 0, s>>>(p);
-    else if (p.dtype == PYC_DTYPE_BF16) token_logprobs_kernel<__nv_bfloat16><<<grid, LT, 0, s>>>(p);
-    else token_logprobs_kernel<__half><<<grid, LT, 0, s>>>(p);
-    B200_CUDA_OK(cudaGetLastError());
-    count_launch();
-    return 0;
+    if (p.dtype == PYC_DTYPE_F32) return launch_scores<float>(p, s);
+    if (p.dtype == PYC_DTYPE_BF16) return launch_scores<__nv_bfloat16>(p, s);
+    return launch_scores<__half>(p, s);
 }
 
 int pyc_b200_token_logprobs_backward(const pyc_b200_token_logprobs_grad_args* a, void* stream) {
@@ -158,15 +565,12 @@ int pyc_b200_token_logprobs_backward(const pyc_b200_token_logprobs_grad_args* a,
     if (!p.row_stride) p.row_stride = p.vocab;
     if (!p.grad_stride) p.grad_stride = p.vocab;
     if (!logits_ok(p.dtype, p.rows, p.vocab, p.row_stride) || !logits_ok(p.dtype, p.rows, p.vocab, p.grad_stride)) return -1;
+    if (!aligned_to(p.logits, p.dtype) || !aligned_to(p.grad_logits, p.dtype)) { set_error("token logprobs backward: logits or gradient are not aligned to their type"); return -1; }
     if (p.grad_logits == p.logits && p.grad_stride != p.row_stride) { set_error("token logprobs backward: in place needs equal strides"); return -1; }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const unsigned grid = static_cast<unsigned>(p.rows);
-    if (p.dtype == PYC_DTYPE_F32) token_logprobs_grad_kernel<float><<<grid, LT, 0, s>>>(p);
-    else if (p.dtype == PYC_DTYPE_BF16) token_logprobs_grad_kernel<__nv_bfloat16><<<grid, LT, 0, s>>>(p);
-    else token_logprobs_grad_kernel<__half><<<grid, LT, 0, s>>>(p);
-    B200_CUDA_OK(cudaGetLastError());
-    count_launch();
-    return 0;
+    if (p.dtype == PYC_DTYPE_F32) return launch_grad<float>(p, s);
+    if (p.dtype == PYC_DTYPE_BF16) return launch_grad<__nv_bfloat16>(p, s);
+    return launch_grad<__half>(p, s);
 }
 
 }  // extern "C"

@@ -219,3 +219,40 @@ def test_gradient_against_differences(backend):
         slope = (loss(vals + e) - loss(vals - e)) / (2 * step)
         # third derivatives of both terms are below 8 in size: step^2 / 6 * 8 * 3; results are good to 2^-16, over 2 * step
         assert np.abs(slope - got[:, j]).max() <= step ** 2 / 6 * 8 * 3 + 2 * 3 * 2.0 ** -16 / (2 * step)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows, vocab", [(3, 60000), (400, 9000)])
+def test_top_of_rows_masked_down_to_a_few_tokens(backend, dtype, rows, vocab):
+    """Fewer unmasked tokens than alternatives asked for: the masked ones follow by index, the lowest value before -inf."""
+    rng = np.random.default_rng(8)
+    low = {F32: -3.4028234663852886e38, BF16: -3.3895313892515355e38, F16: -65504.0}[dtype]
+    x = np.full((rows, vocab), -np.inf)
+    for r in range(rows):
+        x[r, rng.choice(vocab, r % 25, replace=False)] = rng.standard_normal(r % 25)
+        if r % 3 == 1:
+            x[r, rng.choice(vocab, 5, replace=False)] = low
+        if r % 3 == 2:
+            x[r, x[r] == -np.inf] = low
+    tokens = rng.integers(0, vocab, rows)
+    vals, got = _score(backend, dtype, x, tokens, 20)
+    _check(vals, got, tokens, 20)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("vocab", [2048 * 9, 2048 * 40 + 5])
+def test_top_of_rows_whose_large_logits_lie_in_few_threads_shares(backend, dtype, vocab):
+    """Larger logits at the same places of every 2048: more of them than candidates are kept for; and a rising run."""
+    rng = np.random.default_rng(9)
+    x = rng.standard_normal((300, vocab))
+    x[0, np.arange(vocab) % 2048 < 200] += 20.0
+    x[1, np.arange(vocab) % 1024 < 60] += 20.0
+    x[2, np.arange(vocab) % 2048 < 8] = 9.0
+    x[3] = np.arange(vocab) / 4096
+    x[4, 5000:9000] = 30 + np.arange(4000) / 500
+    x[5] = np.where(np.arange(vocab) % 3 == 0, 5.0, -5.0)
+    tokens = rng.integers(0, vocab, 300)
+    vals, got = _score(backend, dtype, x[:8], tokens[:8], 32)            # a cluster per row
+    _check(vals, got, tokens[:8], 32)
+    vals, got = _score(backend, dtype, x, tokens, 32)                    # a CTA per row
+    _check(vals[:8], [g[:8] for g in got], tokens[:8], 32)
