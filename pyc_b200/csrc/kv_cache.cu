@@ -185,13 +185,19 @@ kv_release_kernel(int R, int bs, int block_shift, int num_blocks, int max_blocks
 }
 
 // ------------------------------------------------------------------------------------------------------------ write --
-// One warp per (run, head, keys | values).  Pass 1 finds the run's largest magnitude, pass 2 writes codes; the run's rows
-// are read again in pass 2 (from L1/L2).
+// Bound by reading the 16-bit values and writing the codes, or by latency for single tokens.  One CTA per (group of tokens, head,
+// keys | values) takes the runs that begin in its group one after the other.  A thread holds eight 16-byte vectors, a CTA
+// block_size * head_dim / 2048 warps, so that a whole block's values of a head are loaded at once, kept in registers while
+// their largest magnitude is found, and written as codes: every value is read once.
 template <typename T> struct KvIn;
 template <> struct KvIn<__nv_bfloat16> {
+    static constexpr uint32_t INF = 0x7f80;
+    static __device__ __forceinline__ float widen(uint32_t bits) { return __uint_as_float(bits << 16); }
     static __device__ __forceinline__ void unpack(uint32_t w, float& a, float& b) { a = __uint_as_float(w << 16); b = __uint_as_float(w & 0xffff0000u); }
 };
 template <> struct KvIn<__half> {
+    static constexpr uint32_t INF = 0x7c00;
+    static __device__ __forceinline__ float widen(uint32_t bits) { return __half2float(__ushort_as_half(static_cast<unsigned short>(bits))); }
     static __device__ __forceinline__ void unpack(uint32_t w, float& a, float& b) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w)); a = f.x; b = f.y;
     }
@@ -206,7 +212,22 @@ struct KvWriteParams {
     int tokens, heads, bs, shift, num_blocks, group;
 };
 
-__device__ __forceinline__ float finite_abs(float v) { const float a = fabsf(v); return a <= 3.4028235e38f ? a : 0.0f; }   // NaN compares false
+// Largest magnitude of a thread's values as 16-bit bits (magnitudes order as their bits); FINITE: infinities and NaN left out.
+template <bool FINITE, int VECS>
+__device__ __forceinline__ uint32_t max_bits(const uint4 (&u)[VECS], uint32_t inf) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+        const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t a = w[j] & 0x7fff7fffu;
+            if (FINITE) a = ((a & 0xffffu) < inf ? a & 0xffffu : 0u) | ((a >> 16) < inf ? a & 0xffff0000u : 0u);
+            m = __vmaxu2(m, a);
+        }
+    }
+    return max(m & 0xffffu, m >> 16);
+}
 
 __device__ __forceinline__ uint32_t kv_pack4(float a, float b, float c, float d) {
     const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
@@ -214,76 +235,117 @@ __device__ __forceinline__ uint32_t kv_pack4(float a, float b, float c, float d)
     return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256)
-kv_write_kernel(KvWriteParams p) {
-    constexpr int LPR = D / 8;                   // lanes per row: eight values each
-    constexpr int RPI = 32 / LPR;                // rows per warp and step
+// W: warps per CTA.
+template <typename T, int D, int W>
+__global__ void __launch_bounds__(W * 32, 32 / W)
+kv_write_kernel(const __grid_constant__ KvWriteParams p) {
+    constexpr int THREADS = W * 32, VECS = 8, PER_ROW = D / 8;               // vectors per row of a head
     const int lane = threadIdx.x & 31;
     const int head = blockIdx.y, which = blockIdx.z;
-    const long long first = (static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * p.group;
-    const T* x = static_cast<const T*>(p.x[which]) + head * D;
-    const size_t stride = p.stride[which];
+    const T* x = static_cast<const T*>(which ? p.x[1] : p.x[0]) + head * D;
+    const size_t stride = which ? p.stride[1] : p.stride[0];
+    float* scales = which ? p.scale[1] : p.scale[0];
+    uint8_t* cache = which ? p.cache[1] : p.cache[0];
     const long long pool = static_cast<long long>(p.num_blocks) << p.shift;
-    for (long long t0 = first; t0 < first + p.group && t0 < p.tokens; ++t0) {
-        const long long slot = p.slots[t0];
-        if (slot < 0 || slot >= pool) continue;
-        const int off = static_cast<int>(slot & (p.bs - 1));
-        if (off != 0 && t0 > 0 && p.slots[t0 - 1] == slot - 1) continue;          // inside a run that another token starts
-        const long long block = slot >> p.shift;
-        // length of the run: consecutive slots up to the block's end
-        int n = 1;
-        while (true) {
-            const int i = n + lane;
-            const bool more = off + i < p.bs && t0 + i < p.tokens && p.slots[t0 + i] == slot + i;
-            const unsigned m = __ballot_sync(0xffffffffu, more);
-            if (m == 0xffffffffu) { n += 32; continue; }
-            n += __ffs(~m) - 1;
-            break;
+    const int first = static_cast<int>(blockIdx.x) * p.group, last = min(first + p.group, p.tokens);
+    for (int base = first; base < last; base += 32) {
+        // tokens of these 32 that begin a run (the same in every warp)
+        const int ti = base + lane;
+        long long si = -1;
+        bool leads = false;
+        if (ti < last) {
+            si = __ldg(p.slots + ti);
+            if (si >= 0 && si < pool) leads = (si & (p.bs - 1)) == 0 || ti == 0 || __ldg(p.slots + ti - 1) != si - 1;
         }
-        const int col = (lane % LPR) * 8;
-        float amax = 0.0f;
-        for (int r = lane / LPR; r < n; r += RPI) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + static_cast<size_t>(t0 + r) * stride + col));
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { float a, b; KvIn<T>::unpack(w[j], a, b); amax = fmaxf(amax, fmaxf(finite_abs(a), finite_abs(b))); }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        int e = kv_scale_exponent(amax);
-        float* sp = p.scale[which] + block * p.heads + head;
-        uint8_t* tile = p.cache[which] + (static_cast<size_t>(block) * p.heads + head) * (static_cast<size_t>(p.bs) * D);
-        if (off != 0) {
+        for (unsigned m = __ballot_sync(0xffffffffu, leads); m; m &= m - 1) {
+            const int at = __ffs(m) - 1, t0 = base + at;
+            const long long slot = __shfl_sync(0xffffffffu, si, at), block = slot >> p.shift;
+            const int off = static_cast<int>(slot & (p.bs - 1));
+            float* sp = scales + block * p.heads + head;
             const float old = *sp;
-            e = max(e, kv_exponent_of_scale(old));
-            const float again = old * exp2_int(-e);                              // old scale / new scale
-            if (again != 1.0f) {
-                // codes that the block keeps, rounded again to the grown scale: 16 codes per lane and step
-                for (int i = lane; i < off * D / 16; i += 32) {
-                    uint4 u = reinterpret_cast<uint4*>(tile)[i];
-                    uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 a = e4m3x2_to_float2(w[j] & 0xffffu), b = e4m3x2_to_float2(w[j] >> 16);
-                        w[j] = kv_pack4(a.x * again, a.y * again, b.x * again, b.y * again);
-                    }
-                    reinterpret_cast<uint4*>(tile)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            // the run's tokens: consecutive slots up to the block's end.  A block has one run: where its last slot is the last token's, all are.
+            const int most = min(p.bs - off, p.tokens - t0);
+            int n = most;
+            if (most > 1 && __ldg(p.slots + t0 + most - 1) != slot + most - 1) {
+                n = 1;
+                while (true) {
+                    const int i = n + lane;
+                    const bool more = i < most && __ldg(p.slots + t0 + i) == slot + i;
+                    const unsigned run = __ballot_sync(0xffffffffu, more);
+                    if (run == 0xffffffffu) { n += 32; continue; }
+                    n += __ffs(~run) - 1;
+                    break;
                 }
             }
-        }
-        const float inv = exp2_int(-e);                                          // exact: the scale is a power of two
-        for (int r = lane / LPR; r < n; r += RPI) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + static_cast<size_t>(t0 + r) * stride + col));
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-            float f[8];
+            uint4 u[VECS];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { KvIn<T>::unpack(w[j], f[2 * j], f[2 * j + 1]); f[2 * j] *= inv; f[2 * j + 1] *= inv; }
-            *reinterpret_cast<uint2*>(tile + static_cast<size_t>(off + r) * D + col) = make_uint2(kv_pack4(f[0], f[1], f[2], f[3]), kv_pack4(f[4], f[5], f[6], f[7]));
+            for (int i = 0; i < VECS; ++i) {
+                const int q = i * THREADS + threadIdx.x, r = q / PER_ROW;
+                u[i] = r < n ? __ldg(reinterpret_cast<const uint4*>(x + static_cast<size_t>(t0 + r) * stride) + q % PER_ROW) : make_uint4(0, 0, 0, 0);
+            }
+            auto all = [&](uint32_t m) {                                     // the CTA's largest; also: everybody has read the old scale
+                m = __reduce_max_sync(0xffffffffu, m);
+                if constexpr (W > 1) {
+                    __shared__ uint32_t warp_max[W];
+                    if (lane == 0) warp_max[threadIdx.x >> 5] = m;
+                    __syncthreads();
+#pragma unroll
+                    for (int i = 0; i < W; ++i) m = max(m, warp_max[i]);
+                    __syncthreads();
+                }
+                return m;
+            };
+            uint32_t bits = all(max_bits<false>(u, KvIn<T>::INF));
+            if (bits >= KvIn<T>::INF) bits = all(max_bits<true>(u, KvIn<T>::INF));
+            int e = kv_scale_exponent(KvIn<T>::widen(bits));
+            uint8_t* tile = cache + (static_cast<size_t>(block) * p.heads + head) * (static_cast<size_t>(p.bs) * D);
+            if (off != 0) {
+                e = max(e, kv_exponent_of_scale(old));
+                const float again = old * exp2_int(-e);                      // old scale / new scale
+                if (again != 1.0f) {
+                    // codes that the block keeps, rounded again to the grown scale: 16 codes per thread and step
+                    for (int i = threadIdx.x; i < off * D / 16; i += THREADS) {
+                        uint4 v = reinterpret_cast<uint4*>(tile)[i];
+                        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 a = e4m3x2_to_float2(w[j] & 0xffffu), b = e4m3x2_to_float2(w[j] >> 16);
+                            w[j] = kv_pack4(a.x * again, a.y * again, b.x * again, b.y * again);
+                        }
+                        reinterpret_cast<uint4*>(tile)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+            const float inv = exp2_int(-e);                                  // exact: the scale is a power of two
+            uint2* dst = reinterpret_cast<uint2*>(tile + off * D);
+#pragma unroll
+            for (int i = 0; i < VECS; ++i) {
+                const int q = i * THREADS + threadIdx.x;
+                if (q / PER_ROW < n) {
+                    const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+                    float f[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) { KvIn<T>::unpack(w[j], f[2 * j], f[2 * j + 1]); f[2 * j] *= inv; f[2 * j + 1] *= inv; }
+                    dst[q] = make_uint2(kv_pack4(f[0], f[1], f[2], f[3]), kv_pack4(f[4], f[5], f[6], f[7]));
+                }
+            }
+            if (threadIdx.x == 0) *sp = exp2_int(e);
         }
-        __syncwarp();
-        if (lane == 0) *sp = exp2_int(e);
     }
+}
+
+template <typename T, int D>
+int launch_kv_write(const KvWriteParams& p, cudaStream_t s) {
+    const dim3 grid((p.tokens + p.group - 1) / p.group, p.heads, 2);
+    switch (std::max(1, p.bs * D / 2048)) {
+        case 1: kv_write_kernel<T, D, 1><<<grid, 32, 0, s>>>(p); break;
+        case 2: kv_write_kernel<T, D, 2><<<grid, 64, 0, s>>>(p); break;
+        case 4: kv_write_kernel<T, D, 4><<<grid, 128, 0, s>>>(p); break;
+        default: if constexpr (D == 128) kv_write_kernel<T, D, 8><<<grid, 256, 0, s>>>(p);
+    }
+    B200_CUDA_OK(cudaGetLastError());
+    count_launch();
+    return 0;
 }
 
 bool aligned16(const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; }
@@ -355,19 +417,14 @@ int pyc_b200_kv_write(const pyc_b200_kv_write_args* a, void* stream) {
     p.cache[0] = static_cast<uint8_t*>(a->k_cache); p.cache[1] = static_cast<uint8_t*>(a->v_cache);
     p.scale[0] = a->k_scale; p.scale[1] = a->v_scale;
     p.slots = a->slot_map; p.tokens = a->tokens; p.heads = a->kv_heads; p.bs = a->block_size; p.shift = shift; p.num_blocks = a->num_blocks;
+    // Tokens per CTA: 1 where there are few (every token may be a run of its own), up to a block where there are many (then most
+    // tokens do not begin a run), as long as every SM keeps 32 CTAs to choose from.
+    const long long units = 2ll * a->tokens * a->kv_heads / (static_cast<long long>(sm_count()) * 32);
     p.group = 1;
-    const dim3 grid((a->tokens + 7) / 8, a->kv_heads, 2);
+    while (p.group < a->block_size && p.group * 2 <= units) p.group *= 2;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (a->dtype == PYC_DTYPE_BF16) {
-        if (a->head_dim == 128) kv_write_kernel<__nv_bfloat16, 128><<<grid, 256, 0, s>>>(p);
-        else kv_write_kernel<__nv_bfloat16, 64><<<grid, 256, 0, s>>>(p);
-    } else {
-        if (a->head_dim == 128) kv_write_kernel<__half, 128><<<grid, 256, 0, s>>>(p);
-        else kv_write_kernel<__half, 64><<<grid, 256, 0, s>>>(p);
-    }
-    B200_CUDA_OK(cudaGetLastError());
-    count_launch();
-    return 0;
+    if (a->dtype == PYC_DTYPE_BF16) return a->head_dim == 128 ? launch_kv_write<__nv_bfloat16, 128>(p, s) : launch_kv_write<__nv_bfloat16, 64>(p, s);
+    return a->head_dim == 128 ? launch_kv_write<__half, 128>(p, s) : launch_kv_write<__half, 64>(p, s);
 }
 
 }  // extern "C"
