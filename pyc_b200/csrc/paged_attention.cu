@@ -39,6 +39,7 @@
 
 #include "internal.h"
 #include "paged_attention.cuh"
+#include "paged_attention_chunk.h"
 #include "ptx_sm100.cuh"
 
 namespace b200 {
@@ -555,7 +556,8 @@ extern "C" {
 
 size_t pyc_b200_paged_attention_workspace_bytes(int requests, int max_query, int heads, int kv_heads, int head_dim) {
     if (requests < 1 || max_query < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
-    return WS_COUNTERS + partial_bytes(head_dim);
+    const bool many = static_cast<long long>(max_query) * (heads / kv_heads) > 32;
+    return WS_COUNTERS + (many ? std::max(partial_bytes(head_dim), paged_chunk_partial_bytes(head_dim)) : partial_bytes(head_dim));
 }
 
 int pyc_b200_paged_attention(const pyc_b200_paged_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -602,13 +604,26 @@ int pyc_b200_paged_attention(const pyc_b200_paged_attention_args* a, void* works
     const uint32_t box[3] = {128, static_cast<uint32_t>(GROUP / halves * a->head_dim / 128), 1};
     if (encode_tmap(&tmK, a->k_cache, 1, 3, dims, strides, box, true) != 0 || encode_tmap(&tmV, a->v_cache, 1, 3, dims, strides, box, true) != 0) return -1;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    // Which kernel takes a request goes by its rows (queries times query heads of a key head), decided on the device: up to 8, 16
+    // or 32 rows (the smallest that covers max_query, or one token where that is beyond 32) the one for few rows, more than that the
+    // tcgen05 kernel.  MEASURED
     const long long most = static_cast<long long>(a->max_query) * p.group;
-    p.rows_above = 0; p.rows_upto = INT_MAX;
+    const int few = static_cast<int>(most <= 32 ? most : p.group <= 32 ? p.group : 0);
+    p.cost = 2; p.unsplit = 8;               // an item's end takes about as long as two units' copies; a join takes 4 us, eight units 3
     const bool half = a->dtype == PYC_DTYPE_F16;
+    const int upto = few <= 8 ? 8 : few <= 16 ? 16 : 32;
+    if (few > 0) {
+        p.rows_above = 0; p.rows_upto = upto;
+        int rc;
 #define B200_SHORT(D, NQ) (half ? launch_short<__half, D, NQ>(tmK, tmV, p, halves, s) : launch_short<__nv_bfloat16, D, NQ>(tmK, tmV, p, halves, s))
-    if (a->head_dim == 128) return most <= 8 ? B200_SHORT(128, 1) : most <= 16 ? B200_SHORT(128, 2) : B200_SHORT(128, 4);
-    return most <= 8 ? B200_SHORT(64, 1) : most <= 16 ? B200_SHORT(64, 2) : B200_SHORT(64, 4);
+        if (a->head_dim == 128) rc = upto == 8 ? B200_SHORT(128, 1) : upto == 16 ? B200_SHORT(128, 2) : B200_SHORT(128, 4);
+        else rc = upto == 8 ? B200_SHORT(64, 1) : upto == 16 ? B200_SHORT(64, 2) : B200_SHORT(64, 4);
 #undef B200_SHORT
+        if (rc != 0) return rc;
+    }
+    if (most <= 32) return 0;
+    p.rows_above = few > 0 ? upto : 0; p.rows_upto = INT_MAX;
+    return launch_paged_chunk(a->dtype, a->head_dim, p, a->k_cache, a->v_cache, s);
 }
 
 }  // extern "C"

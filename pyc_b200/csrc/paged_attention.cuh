@@ -3,11 +3,11 @@
 //
 // Work.  An ITEM is (request, tile of query rows, key head): the rows are the request's queries times the query heads of
 // that key head (token-major), so that all of them share the keys.  An item is as many UNITS as it has blocks of
-// UNIT visible keys, at least one, and weighs COST units more, for what its beginning and end take.  All items are laid end
+// UNIT visible keys, at least one, and weighs `cost` units more, for what its beginning and end take.  All items are laid end
 // to end (requests, then tiles, then heads) and every CTA of the grid takes an equal, contiguous stretch of that weight:
 // whatever the lengths, the CTAs finish together, and nothing but the lengths on the device decides it (a captured launch
-// replays with new lengths).  A stretch boundary inside an item's units splits it (one inside its COST moves to its
-// beginning); short items are never split (a join costs 4 us, eight units 3).  Each part leaves its unnormalised sum, its maximum and its weight in the workspace, and the CTA that arrives
+// replays with new lengths).  A stretch boundary inside an item's units splits it (one inside its cost moves to its
+// beginning); short items are never split.  Each part leaves its unnormalised sum, its maximum and its weight in the workspace, and the CTA that arrives
 // last (a counter in the workspace) joins them in the order of the keys -- so results do not depend on who was last.
 #pragma once
 #include <cuda_runtime.h>
@@ -32,6 +32,7 @@ struct PagedParams {
     int rows_above, rows_upto;      // this launch takes the requests with rows_above < queries * group <= rows_upto
     float scale_log2;               // softmax scale * log2(e)
     int causal;
+    int cost, unsplit;              // weight of an item beside its units; items of up to so many units stay whole where the launch has none larger
     int* counters;                  // [CTAs], zero between calls
     float* partials;                // [CTAs][2][tile rows * (head_dim + 2)]
     int* status;
@@ -62,13 +63,11 @@ template <int TILE, int UNIT>
 __device__ __forceinline__ int paged_tile_units(const PagedParams& p, const PagedRequest& q, int t) {
     return max(1, (paged_tile_end<TILE>(p, q, t) + UNIT - 1) / UNIT);
 }
-constexpr int PAGED_UNSPLIT = 8;    // items of up to so many units stay whole where the launch has none larger
-constexpr int PAGED_COST = 2;       // measured: an item's end takes about as long as two units' copies
 // Weight of a request's items of ONE key head.
 template <int TILE, int UNIT>
 __device__ __forceinline__ long long paged_request_weight(const PagedParams& p, const PagedRequest& q) {
     long long n = 0;
-    for (int t = 0; t * TILE < q.rows; ++t) n += paged_tile_units<TILE, UNIT>(p, q, t) + PAGED_COST;
+    for (int t = 0; t * TILE < q.rows; ++t) n += paged_tile_units<TILE, UNIT>(p, q, t) + p.cost;
     return n;
 }
 
@@ -85,11 +84,12 @@ struct PagedCursor {
     int hi;                         // end of the CTA's stretch
     int item;                       // beginning of the current item (below 0 where another CTA has it)
     int r, t, h, units;             // current item and its number of units
+    int cost;
     bool whole;                     // items are not split: one belongs to the CTA with its last position
     PagedRequest q;
     // the CTA's part of the item's units
-    __device__ __forceinline__ int from() const { return whole ? 0 : max(0, -item - PAGED_COST); }
-    __device__ __forceinline__ int to() const { return whole ? (item + PAGED_COST + units <= hi ? units : 0) : min(units, hi - item - PAGED_COST); }
+    __device__ __forceinline__ int from() const { return whole ? 0 : max(0, -item - cost); }
+    __device__ __forceinline__ int to() const { return whole ? (item + cost + units <= hi ? units : 0) : min(units, hi - item - cost); }
 };
 
 // Sums all requests' weights (every CTA for itself: 12 bytes per request out of L2) and finds the item where the CTA's
@@ -116,7 +116,8 @@ __device__ __forceinline__ bool paged_begin(const PagedParams& p, PagedCursor& c
     long long before = 0, total = 0;
 #pragma unroll
     for (int i = 0; i < THREADS / 32; ++i) { const long long x = sh.sums[i]; total += x; if (i < w) before += x; most = max(most, sh.most[i]); }
-    c.whole = most <= PAGED_UNSPLIT;
+    c.whole = most <= p.unsplit;
+    c.cost = p.cost;
     upto += before;
     if (total == 0) return false;
     const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
@@ -142,18 +143,18 @@ __device__ __forceinline__ bool paged_begin(const PagedParams& p, PagedCursor& c
     c.q = paged_request(p, c.r);
     for (c.t = 0;; ++c.t) {
         c.units = paged_tile_units<TILE, UNIT>(p, c.q, c.t);
-        if (at + (c.units + PAGED_COST) * p.kv_heads > 0) break;
-        at += (c.units + PAGED_COST) * p.kv_heads;
+        if (at + (c.units + p.cost) * p.kv_heads > 0) break;
+        at += (c.units + p.cost) * p.kv_heads;
     }
-    c.h = -at / (c.units + PAGED_COST);
-    c.item = at + c.h * (c.units + PAGED_COST);
+    c.h = -at / (c.units + p.cost);
+    c.item = at + c.h * (c.units + p.cost);
     return c.to() > 0;
 }
 // To the CTA's next item; false, and the cursor as it was, when its stretch has no part of it.
 template <int TILE, int UNIT>
 __device__ __forceinline__ bool paged_next(const PagedParams& p, PagedCursor& c) {
-    const int item = c.item + c.units + PAGED_COST;
-    if (item + PAGED_COST >= c.hi) return false;                   // also where there is no further request
+    const int item = c.item + c.units + p.cost;
+    if (item + p.cost >= c.hi) return false;                   // also where there is no further request
     PagedCursor n = c;
     n.item = item;
     if (++n.h == p.kv_heads) {
@@ -173,8 +174,8 @@ __device__ __forceinline__ int paged_cta_of(const PagedShares& s, long long u) {
 }
 
 // CTAs with the item's first and last unit.
-__device__ __forceinline__ int paged_first(const PagedShares& s, const PagedCursor& c) { return paged_cta_of(s, s.lo + c.item + PAGED_COST); }
-__device__ __forceinline__ int paged_last(const PagedShares& s, const PagedCursor& c) { return paged_cta_of(s, s.lo + c.item + PAGED_COST + c.units - 1); }
+__device__ __forceinline__ int paged_first(const PagedShares& s, const PagedCursor& c) { return paged_cta_of(s, s.lo + c.item + c.cost); }
+__device__ __forceinline__ int paged_last(const PagedShares& s, const PagedCursor& c) { return paged_cta_of(s, s.lo + c.item + c.cost + c.units - 1); }
 
 __device__ __forceinline__ float paged_clamp_scale(float s) { return fminf(fmaxf(s, 0x1p-40f), 0x1p72f); }
 
@@ -197,57 +198,60 @@ __device__ __forceinline__ void paged_finish(const PagedParams& p, const PagedCu
 // The parts of split items that this CTA computed (at most two: the item that its stretch begins in and the one that it
 // ends in) have left their sums in its slots.  At the end of its stretch it announces them and joins the items of which all
 // parts are there now.  Announcing late costs nothing -- somebody has to be last -- and keeps the fence and the round trip
-// of the counters out of the way of the copies.  scratch: 2 (TILE + parts * TILE) floats of shared memory, flags: 2 ints.
+// of the counters out of the way of the copies.  scratch: 2 (R + parts * R) floats of shared memory, R = min(TILE, 16); flags: 2 ints.
 template <typename T, int D, int THREADS, int TILE>
 __device__ __forceinline__ void paged_join(const PagedParams& p, const PagedShares& sh, const PagedCursor& c, float* scratch) {
     const int first = paged_first(sh, c), parts = paged_last(sh, c) - first + 1;
-    const int row0 = c.t * TILE, rows = min(TILE, c.q.rows - row0);
     constexpr size_t SLOT = static_cast<size_t>(TILE) * (D + 2);
     auto slot = [&](int i) { return p.partials + (static_cast<size_t>(first + i) * 2 + (i == 0 ? 1 : 0)) * SLOT; };
-    float* row_m = scratch;                                        // [TILE] maximum, [TILE] weight, [parts][rows] maxima, then factors, [parts][rows] weights
-    float* row_l = scratch + TILE;
-    float* f = scratch + 2 * TILE;
-    float* wl = f + parts * rows;
-    for (int e = threadIdx.x; e < parts * rows; e += THREADS) {
-        const float* ml = slot(e / rows) + TILE * D + e % rows;
-        f[e] = __ldcg(ml); wl[e] = __ldcg(ml + TILE);
-    }
-    __syncthreads();
+    constexpr int R = TILE < 16 ? TILE : 16;                       // rows at a time
     const int lane = threadIdx.x & 31;
-    for (int row = threadIdx.x >> 5; row < rows; row += THREADS / 32) {      // one warp per row
-        float m = -INFINITY, l = 0.0f;
-        for (int i = lane; i < parts; i += 32) m = fmaxf(m, f[i * rows + row]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float ref = m == -INFINITY ? 0.0f : m;
-        for (int i = lane; i < parts; i += 32) {
-            const float e = ex2_approx(f[i * rows + row] - ref);
-            f[i * rows + row] = e;
-            l = fmaf(wl[i * rows + row], e, l);
+    for (int r0 = 0; r0 < min(TILE, c.q.rows - c.t * TILE); r0 += R) {
+        const int row0 = c.t * TILE + r0, rows = min(R, c.q.rows - row0);
+        float* row_m = scratch;                                        // [R] maximum, [R] weight, [parts][rows] maxima, then factors, [parts][rows] weights
+        float* row_l = scratch + R;
+        float* f = scratch + 2 * R;
+        float* wl = f + parts * rows;
+        for (int e = threadIdx.x; e < parts * rows; e += THREADS) {
+            const float* ml = slot(e / rows) + TILE * D + r0 + e % rows;
+            f[e] = __ldcg(ml); wl[e] = __ldcg(ml + TILE);
         }
+        __syncthreads();
+        for (int row = threadIdx.x >> 5; row < rows; row += THREADS / 32) {      // one warp per row
+            float m = -INFINITY, l = 0.0f;
+            for (int i = lane; i < parts; i += 32) m = fmaxf(m, f[i * rows + row]);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (lane == 0) { row_m[row] = ref; row_l[row] = l; }
-    }
-    __syncthreads();
-    // the sums: four values per thread and step, sixteen loads in flight
-    for (int e = threadIdx.x; e < rows * (D / 4); e += THREADS) {
-        const int row = e / (D / 4), d = (e % (D / 4)) * 4;
-        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-        for (int i = 0; i < parts; i += 16) {
-            float4 v[16];
-#pragma unroll
-            for (int y = 0; y < 16; ++y) v[y] = i + y < parts ? __ldcg(reinterpret_cast<const float4*>(slot(i + y) + row * D + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int y = 0; y < 16; ++y) {
-                const float w = i + y < parts ? f[(i + y) * rows + row] : 0.0f;
-                o[0] = fmaf(v[y].x, w, o[0]); o[1] = fmaf(v[y].y, w, o[1]); o[2] = fmaf(v[y].z, w, o[2]); o[3] = fmaf(v[y].w, w, o[3]);
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const float ref = m == -INFINITY ? 0.0f : m;
+            for (int i = lane; i < parts; i += 32) {
+                const float e = ex2_approx(f[i * rows + row] - ref);
+                f[i * rows + row] = e;
+                l = fmaf(wl[i * rows + row], e, l);
             }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            if (lane == 0) { row_m[row] = ref; row_l[row] = l; }
         }
-        paged_finish<T, D>(p, c, row0 + row, d, o, row_m[row], row_l[row]);
+        __syncthreads();
+        // the sums: four values per thread and step, sixteen loads in flight
+        for (int e = threadIdx.x; e < rows * (D / 4); e += THREADS) {
+            const int row = e / (D / 4), d = (e % (D / 4)) * 4;
+            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+            for (int i = 0; i < parts; i += 16) {
+                float4 v[16];
+#pragma unroll
+                for (int y = 0; y < 16; ++y) v[y] = i + y < parts ? __ldcg(reinterpret_cast<const float4*>(slot(i + y) + (r0 + row) * D + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int y = 0; y < 16; ++y) {
+                    const float w = i + y < parts ? f[(i + y) * rows + row] : 0.0f;
+                    o[0] = fmaf(v[y].x, w, o[0]); o[1] = fmaf(v[y].y, w, o[1]); o[2] = fmaf(v[y].z, w, o[2]); o[3] = fmaf(v[y].w, w, o[3]);
+                }
+            }
+            paged_finish<T, D>(p, c, row0 + row, d, o, row_m[row], row_l[row]);
+        }
+        __syncthreads();                                               // scratch is free again
     }
-    __syncthreads();                                               // scratch is free again
 }
 
 template <typename T, int D, int THREADS, int TILE>
