@@ -1,20 +1,24 @@
 // Attention over the 8-bit paged cache for many query rows per key head: chunks of prompts, bound by the products.  Items,
-// stretches, split items and their joining are those of paged_attention.cuh; an item's tile has 128 rows (queries times query
-// heads of a key head), a unit 64 keys.
+// stretches, split items and their joining are those of paged_attention.cuh; an item has two tiles of 128 rows (queries times
+// query heads of a key head), a unit 64 keys.
 //
-// 256 threads per CTA, two CTAs per SM, so that one's tensor-core work passes beside the other's softmax:
-//   warp 0      TMEM owner and single-thread MMA issuer
-//                 S[n&1] = Q K_n^T     128 x 64 x D    (tcgen05, f16, S in TMEM, two buffers)
-//                 O     += P_n V_n     128 x D x 64    (P_n from TMEM, where S_n was; V as MN-major operand)
-//   warps 1-3   bring the blocks in: 16-byte loads of e4m3 codes, f16 (exact, two codes per conversion) into the 128-byte-swizzled
-//               operand layout, the next block's loads under way meanwhile.  tcgen05 has no product of e4m3 with 16-bit
-//               operands; splitting the queries into e4m3 terms, as the kernel for few rows does, would spare the keys'
-//               conversion but not the values', and 128 rows share each conversion here
-//   warps 4-7   softmax, one query row per thread; they make the queries' operand first and write the result last
+// One CTA per SM, 14 warps:
+//   warp 0       TMEM owner and single-thread MMA issuer, for both tiles t in turn
+//                  S_t[n&1] = Q_t K_n^T     128 x 64 x D    (tcgen05, f16, S in TMEM, two buffers per tile)
+//                  O_t     += P_n V_n       128 x D x 64    (P_n from TMEM, where S_n was; V as MN-major operand)
+//   warp 1       brings the blocks' codes in (bulk copies, RAW stages), with the scales of their 16-token groups
+//   warps 2-5    codes to f16 operands (exact, two codes per conversion) in the 128-byte-swizzled layout.  tcgen05 has no product of
+//                e4m3 with 16-bit operands; splitting the queries into e4m3 terms, as the kernel for few rows does, would spare the
+//                keys' conversion but not the values', and 256 rows share each conversion here
+//   warps 6-13   softmax, one query row per thread; they make the queries' operand first and write the result last
+// The roles meet at mbarriers only and walk the items each on its own, so that the next item's blocks come in and are converted
+// while the softmax warps write this one's result.  With one tile per CTA and two CTAs per SM, each with its own converters that
+// loaded the codes themselves, 2048-query chunks took 780 us instead of NEW us.
+//
 // Precision is that of paged_attention.cu: queries scaled per row by a power of two and then rounded to f16, which loses
 // what lies below 2^-24 of the row's largest; p' = 2^(score + log2 vs - m) as f16, the softmax's weight sum p' / vs in f32.
-// Values that some row must not see are zero in the operand where they are NaN; the rows that do see one get their NaN at the
-// end (nan_key: the first key, of those that not every row sees, with a NaN in a column).
+// Values that some row must not see are zero in the operand where they are NaN; where that happened, the rows look the NaN
+// that they do see up in the cache at the item's end.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -29,21 +33,24 @@
 namespace b200 {
 namespace {
 
-constexpr int BQ = 128, BK = 64;
-constexpr int THREADS = 256, CONVERTERS = 96;
+constexpr int BQ = 128, TILES = 2, ROWS = BQ * TILES, BK = 64;
+constexpr int MMA_WARP = 0, COPY_WARP = 1, CONVERT_WARP = 2, CONVERT_WARPS = 4, SOFTMAX_WARP = 6;
+constexpr int CONVERTERS = CONVERT_WARPS * 32, THREADS = (SOFTMAX_WARP + 4 * TILES) * 32;
+constexpr int RING = 16;                                 // entries of what is kept per block and per item: more than the roles can be apart
 
 template <int D>
 struct ChunkSmem {
-    static constexpr int Q_BYTES = BQ * D * 2, KV_TILE = BK * D * 2;
-    static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + 2 * KV_TILE;
-    static constexpr int INFO_OFF = V_OFF + 2 * KV_TILE;                 // float4 [4][4]: per block (mod 4) and 16 keys
-    static constexpr int NAN_OFF = INFO_OFF + 256;                       // int [D]
-    static constexpr int BAR_OFF = NAN_OFF + D * 4;                      // q | k full, empty | v full, empty | s full | p full (2 each) | pv done | o done
-    static constexpr int NUM_BARS = 16;
-    static constexpr int SHARES_OFF = BAR_OFF + NUM_BARS * 8 + 16;       // behind the barriers: TMEM address, failure flag
+    static constexpr int RAW = 4;                                        // stages of codes
+    static constexpr int Q_BYTES = BQ * D * 2, KV_TILE = BK * D * 2, RAW_TILE = BK * D;
+    static constexpr int K_OFF = TILES * Q_BYTES, V_OFF = K_OFF + 2 * KV_TILE, RAW_OFF = V_OFF + 2 * KV_TILE;
+    static constexpr int INFO_OFF = RAW_OFF + RAW * 2 * RAW_TILE;        // float4 [RING][4]: per block and 16 keys
+    static constexpr int NAN_OFF = INFO_OFF + RING * 64;                 // int [RING]: per item, whether a NaN value was left out
+    static constexpr int BAR_OFF = NAN_OFF + RING * 4;
+    static constexpr int NUM_BARS = 2 * RAW + 8 + 7 * TILES;             // raw full, empty | k full, empty, v full, empty (2 each) | per tile: q, s full (2), p full (2), pv done, o done
+    static constexpr int SHARES_OFF = BAR_OFF + NUM_BARS * 8 + 16;       // behind the barriers: the TMEM address
     static constexpr int SPLIT_OFF = SHARES_OFF + sizeof(PagedShares);
     static constexpr int BYTES = SPLIT_OFF + 2 * sizeof(PagedCursor) + 16;
-    static_assert((BYTES + 1024) * 2 <= 228 * 1024, "two CTAs per SM");
+    static_assert(BYTES + 1024 <= 228 * 1024 && SHARES_OFF % 8 == 0, "shared memory of an SM");
     static_assert(2 * 16 * (1 + 320) * 4 <= INFO_OFF, "the join's scratch: 16 rows of up to 320 parts");
 };
 
@@ -62,130 +69,174 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
 // 0x80 in each byte that is a NaN code.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+// Untiled copy of `bytes` (a multiple of 16; both addresses 16-byte aligned), counted on `bar`.
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(THREADS, 2)
+__global__ void __launch_bounds__(THREADS, 1)
 paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache) {
     using SM = ChunkSmem<D>;
-    constexpr int HALVES = D / 64, Q_SLAB = BQ * 128, KV_SLAB = BK * 128;
+    constexpr int Q_SLAB = BQ * 128, KV_SLAB = BK * 128, RAW = SM::RAW;
     constexpr uint32_t IDESC_QK = make_idesc(0, 0, 0, 0, BQ, BK), IDESC_PV = make_idesc(0, 0, 0, 1, BQ, D);
-    constexpr uint32_t TMEM_COLS = 256, O_COL = 128;                         // S0 @0, S1 @64, O @128
+    constexpr uint32_t TMEM_COLS = 512, TILE_COLS = 256, O_COL = 128;        // per tile: S0 @0, S1 @64, O @128
     extern __shared__ __align__(1024) uint8_t smem[];
     float4* info = reinterpret_cast<float4*>(smem + SM::INFO_OFF);
-    int* nan_key = reinterpret_cast<int*>(smem + SM::NAN_OFF);
+    int* left_out = reinterpret_cast<int*>(smem + SM::NAN_OFF);
     uint64_t* bar_mem = reinterpret_cast<uint64_t*>(smem + SM::BAR_OFF);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_mem + SM::NUM_BARS);
     PagedShares& shares = *reinterpret_cast<PagedShares*>(smem + SM::SHARES_OFF);
     PagedCursor (&split)[2] = *reinterpret_cast<PagedCursor (*)[2]>(smem + SM::SPLIT_OFF);
     int (&is_split)[2] = *reinterpret_cast<int (*)[2]>(smem + SM::SPLIT_OFF + 2 * sizeof(PagedCursor));
     int* flags = reinterpret_cast<int*>(smem + SM::SPLIT_OFF + 2 * sizeof(PagedCursor) + 8);
-    const uint32_t bar0 = smem_u32(bar_mem);
-    const uint32_t q_full = bar0, k_full = bar0 + 8, k_empty = bar0 + 24, v_full = bar0 + 40, v_empty = bar0 + 56, s_full = bar0 + 72, p_full = bar0 + 88, pv_done = bar0 + 104, o_done = bar0 + 112;
-    const uint32_t sQ = smem_u32(smem), sK = sQ + SM::K_OFF, sV = sQ + SM::V_OFF;
+    const uint32_t raw_full = smem_u32(bar_mem), raw_empty = raw_full + 8 * RAW, k_full = raw_empty + 8 * RAW, k_empty = k_full + 16, v_full = k_full + 32, v_empty = k_full + 48;
+    const uint32_t tile_bars = k_full + 64;              // 7 per tile
+    auto q_full = [&](int t) { return tile_bars + t * 56; };
+    auto s_full = [&](int t, uint32_t st) { return tile_bars + t * 56 + 8 + 8 * st; };
+    auto p_full = [&](int t, uint32_t st) { return tile_bars + t * 56 + 24 + 8 * st; };
+    auto pv_done = [&](int t) { return tile_bars + t * 56 + 40; };
+    auto o_done = [&](int t) { return tile_bars + t * 56 + 48; };
+    const uint32_t sQ = smem_u32(smem), sK = sQ + SM::K_OFF, sV = sQ + SM::V_OFF, sR = sQ + SM::RAW_OFF;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 4);
+        for (int i = 0; i < RAW; ++i) { mbar_init(raw_full + 8 * i, 1); mbar_init(raw_empty + 8 * i, CONVERT_WARPS); }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(k_full + 8 * i, CONVERTERS / 32); mbar_init(k_empty + 8 * i, 1);
-            mbar_init(v_full + 8 * i, CONVERTERS / 32); mbar_init(v_empty + 8 * i, 1);
-            mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, 4);
+            mbar_init(k_full + 8 * i, CONVERT_WARPS); mbar_init(k_empty + 8 * i, 1);
+            mbar_init(v_full + 8 * i, CONVERT_WARPS); mbar_init(v_empty + 8 * i, 1);
         }
-        mbar_init(pv_done, 1); mbar_init(o_done, 1);
+        for (int t = 0; t < TILES; ++t) {
+            mbar_init(q_full(t), 4); mbar_init(pv_done(t), 1); mbar_init(o_done(t), 1);
+            for (int i = 0; i < 2; ++i) { mbar_init(s_full(t, i), 1); mbar_init(p_full(t, i), 4); }
+        }
         fence_barrier_init();
         fence_proxy_async();
         is_split[0] = is_split[1] = 0;
     }
     PagedCursor c;
-    const bool busy = paged_begin<THREADS, BQ, BK>(p, c, shares);
+    const bool busy = paged_begin<THREADS, ROWS, BK>(p, c, shares);
     __syncthreads();
     if (!busy) return;
-    if (warp == 0) { tmem_alloc(smem_u32(tmem_slot), TMEM_COLS); tmem_relinquish(); }
+    if (warp == MMA_WARP) { tmem_alloc(smem_u32(tmem_slot), TMEM_COLS); tmem_relinquish(); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
     uint32_t n = 0;                                      // blocks before this item: every role counts them alike
-    uint32_t items = 0;
+    uint32_t pv = 0, done = 0;                           // blocks and items before this one of this softmax warp's tile (MMA warp: of tile 1, which has no
+                                                         // part in items of up to 128 rows; tile 0 has one in all)
+    bool ok = true;
 
-    for (;; ++items) {
+    for (uint32_t items = 0; ok; ++items) {
         const int j0 = c.from(), j1 = c.to(), blocks = j1 - j0;
-        const int row0 = c.t * BQ, rows = min(BQ, c.q.rows - row0);
-        const int kend = paged_tile_end<BQ>(p, c.q, c.t);
+        const int row0 = c.t * ROWS, rows = min(ROWS, c.q.rows - row0), tiles = rows > BQ ? 2 : 1;
+        const int kend = paged_tile_end<ROWS>(p, c.q, c.t);
         const int all_see = paged_limit(p, c.q, row0 / p.group);             // keys that every row sees
-        if (threadIdx.x < D) nan_key[threadIdx.x] = INT_MAX;
-        __syncthreads();
-        bool ok = true;
 
-        if (warp == 0) {
+        if (warp == MMA_WARP) {
             if (lane == 0) {
                 constexpr uint32_t HI = smem_desc_hi_sw128(1024);
-                const uint32_t q_lo = smem_desc_lo(sQ, 16), k_lo0 = smem_desc_lo(sK, 16), v_lo0 = smem_desc_lo(sV, KV_SLAB);
-                auto issue_qk = [&](uint32_t b) {                            // S[b&1] = Q K_b^T
-                    const uint32_t st = b & 1, k_lo = k_lo0 + st * (SM::KV_TILE >> 4);
+                const uint32_t q_lo0 = smem_desc_lo(sQ, 16), k_lo0 = smem_desc_lo(sK, 16), v_lo0 = smem_desc_lo(sV, KV_SLAB);
+                auto issue_qk = [&](int t, uint32_t b, uint32_t s) {         // S_t[s&1] = Q_t K_b^T
+                    const uint32_t k_lo = k_lo0 + (b & 1) * (SM::KV_TILE >> 4), q_lo = q_lo0 + t * (SM::Q_BYTES >> 4);
 #pragma unroll
                     for (int ks = 0; ks < D / 16; ++ks)
-                        umma_f16(tmem_base + st * BK, smem_desc_join(q_lo + (((ks / 4) * Q_SLAB + (ks % 4) * 32) >> 4), HI),
+                        umma_f16(tmem_base + t * TILE_COLS + (s & 1) * BK, smem_desc_join(q_lo + (((ks / 4) * Q_SLAB + (ks % 4) * 32) >> 4), HI),
                                  smem_desc_join(k_lo + (((ks / 4) * KV_SLAB + (ks % 4) * 32) >> 4), HI), IDESC_QK, ks != 0);
-                    umma_commit(s_full + 8 * st);
-                    umma_commit(k_empty + 8 * st);
+                    umma_commit(s_full(t, s & 1));
+                    if (t + 1 == tiles) umma_commit(k_empty + 8 * (b & 1));
                 };
-                ok = mbar_wait(q_full, items & 1, p.status, 0x63);
-                tc_fence_after();
-                for (int i = 0; i < 2 && i < blocks && ok; ++i) {            // two score blocks in flight before the first P arrives
+                for (int t = 0; t < tiles && ok; ++t) ok = mbar_wait(q_full(t), (t ? done : items) & 1, p.status, 0x63);
+                for (int i = 0; i < 2 && i < blocks && ok; ++i) {            // two score blocks of each tile in flight before the first P arrives
                     const uint32_t b = n + i;
-                    if (!mbar_wait(k_full + 8 * (b & 1), (b >> 1) & 1, p.status, 0x64)) { ok = false; break; }
+                    ok = mbar_wait(k_full + 8 * (b & 1), (b >> 1) & 1, p.status, 0x64);
                     tc_fence_after();
-                    issue_qk(b);
+                    if (ok) for (int t = 0; t < tiles; ++t) issue_qk(t, b, (t ? pv : n) + i);
                 }
                 for (int i = 0; i < blocks && ok; ++i) {
-                    const uint32_t b = n + i, st = b & 1, par = (b >> 1) & 1;
-                    if (!mbar_wait(v_full + 8 * st, par, p.status, 0x65)) { ok = false; break; }
-                    if (!mbar_wait(p_full + 8 * st, par, p.status, 0x66)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint32_t v_lo = v_lo0 + st * (SM::KV_TILE >> 4);
-#pragma unroll
-                    for (int ks = 0; ks < BK / 16; ++ks)
-                        umma_f16_ts(tmem_base + O_COL, tmem_base + st * BK + ks * 8, smem_desc_join(v_lo + ks * (2048 >> 4), HI), IDESC_PV, (i | ks) != 0 ? 1u : 0u);
-                    umma_commit(v_empty + 8 * st);
-                    umma_commit(pv_done);
-                    if (i + 1 == blocks) umma_commit(o_done);
-                    if (i + 2 < blocks) {                                    // S[st] is free once this P V is in the pipe ahead
-                        const uint32_t b2 = b + 2;
-                        if (!mbar_wait(k_full + 8 * (b2 & 1), (b2 >> 1) & 1, p.status, 0x67)) { ok = false; break; }
+                    const uint32_t b = n + i, st = b & 1, par = (b >> 1) & 1, v_lo = v_lo0 + st * (SM::KV_TILE >> 4);
+                    ok = mbar_wait(v_full + 8 * st, par, p.status, 0x65);
+                    for (int t = 0; t < tiles && ok; ++t) {
+                        const uint32_t s = (t ? pv : n) + i;
+                        ok = mbar_wait(p_full(t, s & 1), (s >> 1) & 1, p.status, 0x66);
+                        if (!ok) break;
                         tc_fence_after();
-                        issue_qk(b2);
+#pragma unroll
+                        for (int ks = 0; ks < BK / 16; ++ks)
+                            umma_f16_ts(tmem_base + t * TILE_COLS + O_COL, tmem_base + t * TILE_COLS + (s & 1) * BK + ks * 8, smem_desc_join(v_lo + ks * (2048 >> 4), HI), IDESC_PV, (i | ks) != 0 ? 1u : 0u);
+                        if (t + 1 == tiles) umma_commit(v_empty + 8 * st);
+                        umma_commit(pv_done(t));
+                        if (i + 1 == blocks) umma_commit(o_done(t));
+                        if (i + 2 < blocks) {                                // S_t[st] is free once this P V is in the pipe ahead
+                            ok = mbar_wait(k_full + 8 * st, ((b + 2) >> 1) & 1, p.status, 0x67);
+                            tc_fence_after();
+                            if (ok) issue_qk(t, b + 2, s + 2);
+                        }
                     }
                 }
             }
-            __syncwarp();
-        } else if (warp < 4) {
-            // ---- codes to f16 operands.  Chunk x of a block: 16 codes of token x / (D / 16), from column 16 * (x % (D / 16)).
-            constexpr int PER_ROW = D / 16, CHUNKS = BK * PER_ROW, LOADS = (CHUNKS + CONVERTERS - 1) / CONVERTERS;
-            const int ct = threadIdx.x - 32;
+            ok = __all_sync(0xffffffffu, ok);
+            if (tiles == 2) { pv += blocks; ++done; }
+        } else if (warp == COPY_WARP) {
+            // Lane 4 x + g holds block and scales of 16-token group g of unit base + x; lane 0 issues the copies, of as many tokens at a
+            // time as lie in one block.
+            if (lane == 0) left_out[items % RING] = 0;
             const int* table = p.table + static_cast<size_t>(c.r) * p.max_blocks;
-            uint4 kx[LOADS], vx[LOADS];
-            // lane g < 4 of each warp: block and scales of the block's 16-token group g
+            const int step = min(p.block_size, BK) / 16;                     // groups per copy
             auto block_of = [&](int j) {
-                const int key = j * BK + lane * 16;
-                int id = -1;
-                if (lane < 4 && j < j1 && key < kend) id = __ldg(table + (key >> p.shift));
+                const int unit = j + (lane >> 2), key = unit * BK + (lane & 3) * 16;
+                const int id = unit < j1 && key < kend ? __ldg(table + (key >> p.shift)) : -1;
                 return static_cast<unsigned>(id) < static_cast<unsigned>(p.num_blocks) ? id : -1;
             };
-            auto load = [&](const uint8_t* cache, int j, int id, uint4 (&to)[LOADS]) {
-#pragma unroll
-                for (int i = 0; i < LOADS; ++i) {
-                    const int x = ct + i * CONVERTERS, t = x / PER_ROW, key = j * BK + t;
-                    const int mine = __shfl_sync(0xffffffffu, id, (t >> 4) & 3);
-                    to[i] = make_uint4(0, 0, 0, 0);
-                    if (x < CHUNKS && mine >= 0 && key < kend)
-                        to[i] = __ldg(reinterpret_cast<const uint4*>(cache + ((static_cast<size_t>(mine) * p.kv_heads + c.h) * p.block_size + (key & (p.block_size - 1))) * D) + x % PER_ROW);
+            int id_next = block_of(j0);
+            for (int j = j0; j < j1 && ok; j += 8) {
+                const int id = id_next;
+                id_next = block_of(j + 8);
+                float ks = 0.0f, vs = 1.0f;
+                if (id >= 0) {
+                    const size_t at = static_cast<size_t>(id) * p.kv_heads + c.h;
+                    ks = paged_clamp_scale(__ldg(p.k_scale + at)); vs = paged_clamp_scale(__ldg(p.v_scale + at));
                 }
-            };
-            auto store = [&](uint32_t tile, const uint4 (&from)[LOADS]) {
+                const float4 about = make_float4(ks, log2f(vs), 1.0f / vs, 0.0f);
+                for (int x = 0; x < 8 && j + x < j1; ++x) {
+                    const uint32_t b = n + (j + x - j0), st = b % RAW;
+                    ok = __all_sync(0xffffffffu, mbar_wait(raw_empty + 8 * st, ((b / RAW) & 1) ^ 1, p.status, 0x68));
+                    if (!ok) break;
+                    if ((lane >> 2) == x) info[(b % RING) * 4 + (lane & 3)] = about;
+                    __syncwarp();
+                    uint32_t bytes = 0;
+                    for (int g = 0; g < 4; g += step) {
+                        const int mine = __shfl_sync(0xffffffffu, id, x * 4 + g);
+                        if (mine >= 0) bytes += step * 16 * D * 2;
+                    }
+                    if (lane == 0) mbar_arrive_expect_tx(raw_full + 8 * st, bytes);
+                    for (int g = 0; g < 4; g += step) {
+                        const int mine = __shfl_sync(0xffffffffu, id, x * 4 + g);
+                        if (mine >= 0 && lane == 0) {
+                            const int key = (j + x) * BK + g * 16;
+                            const size_t at = ((static_cast<size_t>(mine) * p.kv_heads + c.h) * p.block_size + (key & (p.block_size - 1))) * D;
+                            const uint32_t dst = sR + st * 2 * SM::RAW_TILE + g * 16 * D;
+                            bulk_copy(dst, k_cache + at, step * 16 * D, raw_full + 8 * st);
+                            bulk_copy(dst + SM::RAW_TILE, v_cache + at, step * 16 * D, raw_full + 8 * st);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        } else if (warp < SOFTMAX_WARP) {
+            // ---- codes to f16 operands.  Chunk x of a block: 16 codes of token x / (D / 16), from column 16 * (x % (D / 16)).
+            constexpr int PER_ROW = D / 16, LOADS = BK * PER_ROW / CONVERTERS;
+            const int ct = threadIdx.x - CONVERT_WARP * 32;
+            auto convert = [&](uint32_t tile, const uint4 (&from)[LOADS]) {
 #pragma unroll
                 for (int i = 0; i < LOADS; ++i) {
                     const int x = ct + i * CONVERTERS, t = x / PER_ROW, col = (x % PER_ROW) * 2;      // in 16-byte chunks of 8 f16
-                    if (x >= CHUNKS) break;
                     uint32_t h[8];
                     e4m3x4_to_f16x4(from[i].x, h[0], h[1]); e4m3x4_to_f16x4(from[i].y, h[2], h[3]);
                     e4m3x4_to_f16x4(from[i].z, h[4], h[5]); e4m3x4_to_f16x4(from[i].w, h[6], h[7]);
@@ -194,59 +245,60 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                     sts128(line + ((((col & 7) + 1) ^ sw) << 4), h[4], h[5], h[6], h[7]);
                 }
             };
-            int id = block_of(j0);
-            load(k_cache, j0, id, kx);
-            load(v_cache, j0, id, vx);
             for (int j = j0; j < j1 && ok; ++j) {
-                const uint32_t b = n + (j - j0), st = b & 1, par = ((b >> 1) & 1) ^ 1;
-                const int id_next = block_of(j + 1);
-                float ks = 0.0f, vs = 1.0f;
-                if (id >= 0) {
-                    const size_t at = static_cast<size_t>(id) * p.kv_heads + c.h;
-                    ks = paged_clamp_scale(__ldg(p.k_scale + at)); vs = paged_clamp_scale(__ldg(p.v_scale + at));
-                }
-                ok = __all_sync(0xffffffffu, mbar_wait(k_empty + 8 * st, par, p.status, 0x68));
+                const uint32_t b = n + (j - j0), st = b & 1, par = ((b >> 1) & 1) ^ 1, raw = sR + (b % RAW) * 2 * SM::RAW_TILE;
+                ok = __all_sync(0xffffffffu, mbar_wait(raw_full + 8 * (b % RAW), (b / RAW) & 1, p.status, 0x69));
                 if (!ok) break;
-                if (warp == 1 && lane < 4) info[(b & 3) * 4 + lane] = make_float4(ks, log2f(vs), 1.0f / vs, 0.0f);
-                store(sK + st * SM::KV_TILE, kx);
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(k_full + 8 * st);
-                load(k_cache, j + 1, id_next, kx);
-                if ((j + 1) * BK > all_see) {
-                    // keys that some row does not see: NaN values leave the operand, and the first key with one is kept for each column
+                uint4 kx[LOADS], vx[LOADS];
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) { kx[i] = lds128(raw + (ct + i * CONVERTERS) * 16); vx[i] = lds128(raw + SM::RAW_TILE + (ct + i * CONVERTERS) * 16); }
+                const bool cut = (j + 1) * BK > all_see;
+                const float4 in[4] = {info[(b % RING) * 4], info[(b % RING) * 4 + 1], info[(b % RING) * 4 + 2], info[(b % RING) * 4 + 3]};
+                if (cut || in[0].x == 0.0f || in[1].x == 0.0f || in[2].x == 0.0f || in[3].x == 0.0f) {
+                    // tokens behind the last key and blocks outside the pool: whatever lies there becomes zero, and so do NaN values that some
+                    // row does not see (0 * NaN would reach it)
+                    bool nan = false;
 #pragma unroll
                     for (int i = 0; i < LOADS; ++i) {
-                        const int x = ct + i * CONVERTERS, key = j * BK + x / PER_ROW;
+                        const int t = (ct + i * CONVERTERS) / PER_ROW;
+                        const bool none = j * BK + t >= kend || (t < 16 ? in[0].x : t < 32 ? in[1].x : t < 48 ? in[2].x : in[3].x) == 0.0f;
                         uint32_t w[4] = {vx[i].x, vx[i].y, vx[i].z, vx[i].w};
 #pragma unroll
                         for (int y = 0; y < 4; ++y) {
-                            const uint32_t z = nan_bytes(w[y]);
-                            if (z != 0 && x < CHUNKS) {
-                                for (int e = 0; e < 4; ++e) if (z & (0x80u << (8 * e))) atomicMin(nan_key + (x % PER_ROW) * 16 + y * 4 + e, key);
-                                w[y] &= ~((z >> 7) * 0xffu);
-                            }
+                            if (none) w[y] = 0;
+                            const uint32_t z = cut ? nan_bytes(w[y]) : 0u;
+                            nan |= z != 0;
+                            w[y] &= ~((z >> 7) * 0xffu);
                         }
                         vx[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                        if (none) kx[i] = make_uint4(0, 0, 0, 0);
                     }
+                    if (nan) left_out[items % RING] = 1;
                 }
-                ok = __all_sync(0xffffffffu, mbar_wait(v_empty + 8 * st, par, p.status, 0x69));
+                __syncwarp();
+                if (lane == 0) mbar_arrive(raw_empty + 8 * (b % RAW));
+                ok = __all_sync(0xffffffffu, mbar_wait(k_empty + 8 * st, par, p.status, 0x6a));
                 if (!ok) break;
-                store(sV + st * SM::KV_TILE, vx);
+                convert(sK + st * SM::KV_TILE, kx);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(k_full + 8 * st);
+                ok = __all_sync(0xffffffffu, mbar_wait(v_empty + 8 * st, par, p.status, 0x6b));
+                if (!ok) break;
+                convert(sV + st * SM::KV_TILE, vx);
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(v_full + 8 * st);
-                load(v_cache, j + 1, id_next, vx);
-                id = id_next;
             }
-        } else {
-            const int wq = warp & 3, row = wq * 32 + lane;
-            const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(wq * 32) << 16);
-            const int token = (row0 + min(row, rows - 1)) / p.group, head = c.h * p.group + (row0 + min(row, rows - 1) - token * p.group);
+        } else if ((warp - SOFTMAX_WARP) / 4 < tiles) {
+            const int t = (warp - SOFTMAX_WARP) / 4, wq = warp & 3, in_tile = wq * 32 + lane, row = t * BQ + in_tile;
+            const uint32_t lane_addr = tmem_base + t * TILE_COLS + (static_cast<uint32_t>(wq * 32) << 16);
+            const int at_row = row0 + min(row, rows - 1), token = at_row / p.group, head = c.h * p.group + (at_row - token * p.group);
             const int lim = paged_limit(p, c.q, token);
-            // ---- this thread's query row, scaled to [1, 2) by a power of two, as f16 operand
+            // ---- this thread's query row, scaled to [1, 2) by a power of two, as f16 operand.  The last products with the previous item's
+            // operand are over: their scores have been read.
             float qs;
-            bool finite = true;                                              // one that is not becomes zeros, and NaN at the end if it sees a key
+            bool finite = true;                                              // a row that is not becomes zeros, and NaN at the end if it sees a key
             {
                 const T* src = static_cast<const T*>(p.q) + (static_cast<size_t>(c.q.start) + token) * p.q_stride + static_cast<size_t>(head) * D;
                 float amax = 0.0f;
@@ -272,17 +324,18 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                     uint32_t h[4];
 #pragma unroll
                     for (int y = 0; y < 4; ++y) { const float2 f = wide2<T>(w[y]); h[y] = finite ? pack_f16(f.x * down, f.y * down) : 0u; }
-                    sts128(sQ + (i >> 3) * Q_SLAB + row * 128 + (((i & 7) ^ (row & 7)) << 4), h[0], h[1], h[2], h[3]);
+                    sts128(sQ + t * SM::Q_BYTES + (i >> 3) * Q_SLAB + in_tile * 128 + (((i & 7) ^ (in_tile & 7)) << 4), h[0], h[1], h[2], h[3]);
                 }
                 fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(q_full);
+                if (lane == 0) mbar_arrive(q_full(t));
             }
             float m = -INFINITY, l = 0.0f;
             const int warp_sees = __shfl_sync(0xffffffffu, lim, 0);          // keys that every row of the warp sees
             for (int i = 0; i < blocks && ok; ++i) {
-                const uint32_t b = n + i, st = b & 1, s_addr = lane_addr + st * BK;
-                if (!mbar_wait(s_full + 8 * st, (b >> 1) & 1, p.status, 0x6a)) { ok = false; break; }
+                const uint32_t b = n + i, s = pv + i, s_addr = lane_addr + (s & 1) * BK;
+                ok = __all_sync(0xffffffffu, mbar_wait(s_full(t, s & 1), (s >> 1) & 1, p.status, 0x6c));
+                if (!ok) break;
                 tc_fence_after();
                 const int k0 = (j0 + i) * BK;
                 uint32_t r[64];
@@ -290,7 +343,7 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                 tmem_ld_32x32(s_addr + 32, reinterpret_cast<uint32_t (&)[32]>(r[32]));
                 float4 in[4];
 #pragma unroll
-                for (int g = 0; g < 4; ++g) in[g] = info[(b & 3) * 4 + g];
+                for (int g = 0; g < 4; ++g) in[g] = info[(b % RING) * 4 + g];
                 tmem_ld_wait();
                 const bool gone = in[0].x == 0.0f || in[1].x == 0.0f || in[2].x == 0.0f || in[3].x == 0.0f;
                 if (k0 + BK > warp_sees || gone) {
@@ -337,7 +390,8 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                 // O is touched only when some row of the warp moved its reference, and only then must the previous P V have finished
                 // (the one before it has, for this block's scores came behind it, and this block's cannot: the parity says which)
                 if (i > 0 && __any_sync(0xffffffffu, move)) {
-                    if (!mbar_wait(pv_done, (b - 1) & 1, p.status, 0x6b)) { ok = false; break; }
+                    ok = __all_sync(0xffffffffu, mbar_wait(pv_done(t), (s - 1) & 1, p.status, 0x6d));
+                    if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
                     for (int x = 0; x < D / 32; ++x) {
@@ -353,18 +407,33 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + 8 * st);
+                if (lane == 0) mbar_arrive(p_full(t, s & 1));
             }
             // the last P V has a barrier of its own, one completion per item: this warp may come to it when any number have completed
-            if (ok) ok = mbar_wait(o_done, items & 1, p.status, 0x6c);
-            ok = __all_sync(0xffffffffu, ok);
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), done & 1, p.status, 0x6e));
             if (ok) {
                 tc_fence_after();
                 const bool whole = j0 == 0 && j1 == c.units;
-                float* part = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + (j0 == 0 ? 1 : 0)) * (static_cast<size_t>(BQ) * (D + 2));
+                float* part = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + (j0 == 0 ? 1 : 0)) * (static_cast<size_t>(ROWS) * (D + 2));
                 const float ref = m == -INFINITY ? 0.0f : m;
                 if (!finite && l > 0.0f) l = __int_as_float(0x7fffffff);
-#pragma unroll 1
+                // columns of NaN values that were left out and that this row sees
+                uint32_t nan_cols[D / 32];
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x) nan_cols[x] = 0;
+                if (*reinterpret_cast<volatile int*>(left_out + items % RING)) {
+                    for (int key = max(j0, all_see / BK) * BK; key < min(lim, j1 * BK); ++key) {
+                        const int id = __ldg(p.table + static_cast<size_t>(c.r) * p.max_blocks + (key >> p.shift));
+                        if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.num_blocks)) continue;
+                        const uint32_t* v = reinterpret_cast<const uint32_t*>(v_cache + ((static_cast<size_t>(id) * p.kv_heads + c.h) * p.block_size + (key & (p.block_size - 1))) * D);
+#pragma unroll
+                        for (int y = 0; y < D / 4; ++y) {
+                            const uint32_t z = nan_bytes(__ldg(v + y)) >> 7;
+                            nan_cols[y / 8] |= ((z & 1u) | ((z >> 7) & 2u) | ((z >> 14) & 4u) | ((z >> 21) & 8u)) << (4 * (y % 8));
+                        }
+                    }
+                }
+#pragma unroll
                 for (int x = 0; x < D / 32; ++x) {
                     uint32_t r[32];
                     tmem_ld_32x32(lane_addr + O_COL + x * 32, r);
@@ -376,7 +445,7 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
                                 v[e] = l == 0.0f ? 0.0f : __uint_as_float(r[y + e]);      // no key seen: whatever the products left
-                                if (nan_key[x * 32 + y + e] < lim) v[e] = __int_as_float(0x7fffffff);
+                                if (nan_cols[x] >> (y + e) & 1u) v[e] = __int_as_float(0x7fffffff);
                             }
                             if (whole) paged_finish<T, D>(p, c, row0 + row, x * 32 + y, v, ref, l);
                             else {
@@ -388,23 +457,22 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                     }
                     __syncwarp();
                 }
-                if (!whole && row < rows) { __stcg(part + BQ * D + row, m); __stcg(part + BQ * (D + 1) + row, l); }
+                if (!whole && row < rows) { __stcg(part + ROWS * D + row, m); __stcg(part + ROWS * (D + 1) + row, l); }
+                tc_fence_before();
+                __syncwarp();
             }
-            tc_fence_before();
+            pv += blocks; ++done;
         }
         n += blocks;
-        const bool whole = j0 == 0 && j1 == c.units;
-        if (!whole && threadIdx.x == 0) { split[j0 == 0 ? 1 : 0] = c; is_split[j0 == 0 ? 1 : 0] = 1; }
-        // the next item when every role has left this one: Q, S, O and the counters are free.  A role whose wait ran out ends the CTA's work.
-        if (__syncthreads_or(!ok)) break;
-        tc_fence_after();
-        if (!paged_next<BQ, BK>(p, c)) break;
+        if (threadIdx.x == 0 && (j0 != 0 || j1 != c.units)) { split[j0 == 0 ? 1 : 0] = c; is_split[j0 == 0 ? 1 : 0] = 1; }
+        if (!paged_next<ROWS, BK>(p, c)) break;
     }
+    tc_fence_before();
     __syncthreads();
     if (*reinterpret_cast<volatile int*>(p.status) != ST_OK) for (int i = 0; i < 2000; ++i) __nanosleep(1000);       // let what is in flight land
     tc_fence_after();
-    if (warp == 0) tmem_dealloc(tmem_base, TMEM_COLS);
-    paged_announce<T, D, THREADS, BQ>(p, shares, split, is_split, flags, reinterpret_cast<float*>(smem));
+    if (warp == MMA_WARP) tmem_dealloc(tmem_base, TMEM_COLS);
+    paged_announce<T, D, THREADS, ROWS>(p, shares, split, is_split, flags, reinterpret_cast<float*>(smem));
 }
 
 template <typename T, int D>
@@ -419,8 +487,8 @@ int launch(const PagedParams& p, const void* k_cache, const void* v_cache, cudaS
 
 }  // namespace
 
-int paged_chunk_ctas() { return std::min(sm_count() * 2, 320); }
-size_t paged_chunk_partial_bytes(int head_dim) { return static_cast<size_t>(paged_chunk_ctas()) * 2 * BQ * (head_dim + 2) * sizeof(float); }
+int paged_chunk_ctas() { return std::min(sm_count(), 320); }
+size_t paged_chunk_partial_bytes(int head_dim) { return static_cast<size_t>(paged_chunk_ctas()) * 2 * ROWS * (head_dim + 2) * sizeof(float); }
 
 int launch_paged_chunk(pyc_dtype dtype, int head_dim, PagedParams p, const void* k_cache, const void* v_cache, cudaStream_t s) {
     // an item's queries, first blocks and result take about as long as ten units of 64 keys (0.5 us each with two CTAs on the SM)
