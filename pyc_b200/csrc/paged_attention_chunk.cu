@@ -63,6 +63,9 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) { const __half2 h
 template <typename T> __device__ __forceinline__ float2 wide2(uint32_t w);
 template <> __device__ __forceinline__ float2 wide2<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 template <> __device__ __forceinline__ float2 wide2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <typename T> __device__ __forceinline__ uint32_t narrow2(float a, float b);
+template <> __device__ __forceinline__ uint32_t narrow2<__nv_bfloat16>(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+template <> __device__ __forceinline__ uint32_t narrow2<__half>(float a, float b) { return pack_f16(a, b); }
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
@@ -240,9 +243,12 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                     uint32_t h[8];
                     e4m3x4_to_f16x4(from[i].x, h[0], h[1]); e4m3x4_to_f16x4(from[i].y, h[2], h[3]);
                     e4m3x4_to_f16x4(from[i].z, h[4], h[5]); e4m3x4_to_f16x4(from[i].w, h[6], h[7]);
-                    const uint32_t line = tile + (col >> 3) * KV_SLAB + t * 128, sw = t & 7;
-                    sts128(line + (((col & 7) ^ sw) << 4), h[0], h[1], h[2], h[3]);
-                    sts128(line + ((((col & 7) + 1) ^ sw) << 4), h[4], h[5], h[6], h[7]);
+                    // eight threads write one token's line in both 64-column slabs, which lie on the same banks: those of the second slab
+                    // write their odd chunk first
+                    const uint32_t line = tile + (col >> 3) * KV_SLAB + t * 128, sw = t & 7, odd = (col >> 3) & 1;
+                    const uint32_t first = ((col & 7) + odd) ^ sw, second = first ^ 1;
+                    sts128(line + (first << 4), odd ? h[4] : h[0], odd ? h[5] : h[1], odd ? h[6] : h[2], odd ? h[7] : h[3]);
+                    sts128(line + (second << 4), odd ? h[0] : h[4], odd ? h[1] : h[5], odd ? h[2] : h[6], odd ? h[3] : h[7]);
                 }
             };
             for (int j = j0; j < j1 && ok; ++j) {
@@ -302,10 +308,12 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
             {
                 const T* src = static_cast<const T*>(p.q) + (static_cast<size_t>(c.q.start) + token) * p.q_stride + static_cast<size_t>(head) * D;
                 float amax = 0.0f;
-#pragma unroll 4
+                uint4 u[D / 8];
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+#pragma unroll
                 for (int i = 0; i < D / 8; ++i) {
-                    const uint4 u = __ldg(reinterpret_cast<const uint4*>(src) + i);
-                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                    const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
                         const float2 f = wide2<T>(w[y]);
@@ -317,10 +325,9 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                 const int e = amax > 0.0f && finite ? min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -126), 126) : 0;
                 const float down = exp2_int(-e);
                 qs = exp2_int(e) * p.scale_log2;
-#pragma unroll 4
+#pragma unroll
                 for (int i = 0; i < D / 8; ++i) {
-                    const uint4 u = __ldg(reinterpret_cast<const uint4*>(src) + i);
-                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                    const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
                     uint32_t h[4];
 #pragma unroll
                     for (int y = 0; y < 4; ++y) { const float2 f = wide2<T>(w[y]); h[y] = finite ? pack_f16(f.x * down, f.y * down) : 0u; }
@@ -417,6 +424,8 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                 float* part = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + (j0 == 0 ? 1 : 0)) * (static_cast<size_t>(ROWS) * (D + 2));
                 const float ref = m == -INFINITY ? 0.0f : m;
                 if (!finite && l > 0.0f) l = __int_as_float(0x7fffffff);
+                T* out = static_cast<T*>(p.out) + (static_cast<size_t>(c.q.start) + token) * p.out_stride + static_cast<size_t>(head) * D;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 // columns of NaN values that were left out and that this row sees
                 uint32_t nan_cols[D / 32];
 #pragma unroll
@@ -447,7 +456,7 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                                 v[e] = l == 0.0f ? 0.0f : __uint_as_float(r[y + e]);      // no key seen: whatever the products left
                                 if (nan_cols[x] >> (y + e) & 1u) v[e] = __int_as_float(0x7fffffff);
                             }
-                            if (whole) paged_finish<T, D>(p, c, row0 + row, x * 32 + y, v, ref, l);
+                            if (whole) *reinterpret_cast<uint4*>(out + x * 32 + y) = make_uint4(narrow2<T>(v[0] * inv, v[1] * inv), narrow2<T>(v[2] * inv, v[3] * inv), narrow2<T>(v[4] * inv, v[5] * inv), narrow2<T>(v[6] * inv, v[7] * inv));
                             else {
                                 float* dst = part + row * D + x * 32 + y;
                                 __stcg(reinterpret_cast<float4*>(dst), make_float4(v[0], v[1], v[2], v[3]));
@@ -457,6 +466,7 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                     }
                     __syncwarp();
                 }
+                if (whole && row < rows && p.lse) p.lse[(static_cast<size_t>(c.q.start) + token) * (static_cast<size_t>(p.group) * p.kv_heads) + head] = l == 0.0f ? -INFINITY : (ref + log2f(l)) * 0.69314718055994531f;
                 if (!whole && row < rows) { __stcg(part + ROWS * D + row, m); __stcg(part + ROWS * (D + 1) + row, l); }
                 tc_fence_before();
                 __syncwarp();
