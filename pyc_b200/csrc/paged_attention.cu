@@ -523,7 +523,7 @@ paged_short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             for (int i = SM::EARLY; i < S && i < c.to(); ++i) copy(i, stage(i));
         }
     }
-    paged_announce<T, D, THREADS, TILE>(p, shares, split, is_split, flags, reinterpret_cast<float*>(smem));
+    paged_announce<T, D, THREADS, TILE>(p, shares, split, is_split, flags);
     if (!ok) for (int i = 0; i < 2000; ++i) __nanosleep(1000);               // a wait has run out: let what is in flight land
 }
 

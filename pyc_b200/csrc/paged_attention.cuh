@@ -198,64 +198,80 @@ __device__ __forceinline__ void paged_finish(const PagedParams& p, const PagedCu
 // The parts of split items that this CTA computed (at most two: the item that its stretch begins in and the one that it
 // ends in) have left their sums in its slots.  At the end of its stretch it announces them and joins the items of which all
 // parts are there now.  Announcing late costs nothing -- somebody has to be last -- and keeps the fence and the round trip
-// of the counters out of the way of the copies.  scratch: 2 (R + parts * R) floats of shared memory, R = min(TILE, 16); flags: 2 ints.
+// of the counters out of the way of the copies.  flags: 2 ints of shared memory.
 template <typename T, int D, int THREADS, int TILE>
-__device__ __forceinline__ void paged_join(const PagedParams& p, const PagedShares& sh, const PagedCursor& c, float* scratch) {
+__device__ __forceinline__ void paged_join(const PagedParams& p, const PagedShares& sh, const PagedCursor& c) {
     const int first = paged_first(sh, c), parts = paged_last(sh, c) - first + 1;
     constexpr size_t SLOT = static_cast<size_t>(TILE) * (D + 2);
     auto slot = [&](int i) { return p.partials + (static_cast<size_t>(first + i) * 2 + (i == 0 ? 1 : 0)) * SLOT; };
-    constexpr int R = TILE < 16 ? TILE : 16;                       // rows at a time
-    const int lane = threadIdx.x & 31;
-    for (int r0 = 0; r0 < min(TILE, c.q.rows - c.t * TILE); r0 += R) {
-        const int row0 = c.t * TILE + r0, rows = min(R, c.q.rows - row0);
-        float* row_m = scratch;                                        // [R] maximum, [R] weight, [parts][rows] maxima, then factors, [parts][rows] weights
-        float* row_l = scratch + R;
-        float* f = scratch + 2 * R;
-        float* wl = f + parts * rows;
-        for (int e = threadIdx.x; e < parts * rows; e += THREADS) {
-            const float* ml = slot(e / rows) + TILE * D + r0 + e % rows;
-            f[e] = __ldcg(ml); wl[e] = __ldcg(ml + TILE);
-        }
-        __syncthreads();
-        for (int row = threadIdx.x >> 5; row < rows; row += THREADS / 32) {      // one warp per row
-            float m = -INFINITY, l = 0.0f;
-            for (int i = lane; i < parts; i += 32) m = fmaxf(m, f[i * rows + row]);
+    // One warp per row; lane i has the maxima and weights of parts i, i + 32, .. and the values D / 32 i .. of the sums.  What is
+    // asked for at once: the maxima and weights, and the sums of BATCH parts, of AT_ONCE rows (large tiles are split in two or
+    // three, small ones in up to hundreds).
+    constexpr int VPL = D / 32, AT_ONCE = TILE >= 64 ? 4 : 1, BATCH = TILE >= 64 ? 4 : 16;
+    const int lane = threadIdx.x & 31, rows = min(TILE, c.q.rows - c.t * TILE);
+    for (int r0 = (threadIdx.x >> 5) * AT_ONCE; r0 < rows; r0 += THREADS / 32 * AT_ONCE) {
+        float mi[AT_ONCE], li[AT_ONCE], m[AT_ONCE], l[AT_ONCE], o[AT_ONCE][VPL], v[AT_ONCE][BATCH][VPL];
+        auto weights = [&](int i0) {         // of parts i0 + lane
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float ref = m == -INFINITY ? 0.0f : m;
-            for (int i = lane; i < parts; i += 32) {
-                const float e = ex2_approx(f[i * rows + row] - ref);
-                f[i * rows + row] = e;
-                l = fmaf(wl[i * rows + row], e, l);
+            for (int x = 0; x < AT_ONCE; ++x) {
+                const float* ml = slot(min(i0 + lane, parts - 1)) + TILE * D + min(r0 + x, rows - 1);
+                mi[x] = __ldcg(ml); li[x] = __ldcg(ml + TILE);
+                if (i0 + lane >= parts) { mi[x] = -INFINITY; li[x] = 0.0f; }
             }
+        };
+        auto sums = [&](int i) {             // of parts i .. i + BATCH - 1 (beyond the last: the last's)
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if (lane == 0) { row_m[row] = ref; row_l[row] = l; }
-        }
-        __syncthreads();
-        // the sums: four values per thread and step, sixteen loads in flight
-        for (int e = threadIdx.x; e < rows * (D / 4); e += THREADS) {
-            const int row = e / (D / 4), d = (e % (D / 4)) * 4;
-            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-            for (int i = 0; i < parts; i += 16) {
-                float4 v[16];
+            for (int x = 0; x < AT_ONCE; ++x)
 #pragma unroll
-                for (int y = 0; y < 16; ++y) v[y] = i + y < parts ? __ldcg(reinterpret_cast<const float4*>(slot(i + y) + (r0 + row) * D + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (int y = 0; y < 16; ++y) {
-                    const float w = i + y < parts ? f[(i + y) * rows + row] : 0.0f;
-                    o[0] = fmaf(v[y].x, w, o[0]); o[1] = fmaf(v[y].y, w, o[1]); o[2] = fmaf(v[y].z, w, o[2]); o[3] = fmaf(v[y].w, w, o[3]);
+                for (int y = 0; y < BATCH; ++y) {
+                    const float* src = slot(min(i + y, parts - 1)) + min(r0 + x, rows - 1) * D + lane * VPL;
+                    if constexpr (VPL == 4) { const float4 u = __ldcg(reinterpret_cast<const float4*>(src)); v[x][y][0] = u.x; v[x][y][1] = u.y; v[x][y][2] = u.z; v[x][y][3] = u.w; }
+                    else { const float2 u = __ldcg(reinterpret_cast<const float2*>(src)); v[x][y][0] = u.x; v[x][y][1] = u.y; }
                 }
-            }
-            paged_finish<T, D>(p, c, row0 + row, d, o, row_m[row], row_l[row]);
+        };
+        weights(0);
+        sums(0);
+#pragma unroll
+        for (int x = 0; x < AT_ONCE; ++x) {
+            m[x] = mi[x]; l[x] = 0.0f;
+            for (int i = lane + 32; i < parts; i += 32) m[x] = fmaxf(m[x], __ldcg(slot(i) + TILE * D + min(r0 + x, rows - 1)));
+#pragma unroll
+            for (int y = 16; y > 0; y >>= 1) m[x] = fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], y));
+            if (m[x] == -INFINITY) m[x] = 0.0f;
+#pragma unroll
+            for (int y = 0; y < VPL; ++y) o[x][y] = 0.0f;
         }
-        __syncthreads();                                               // scratch is free again
+#pragma unroll 1
+        for (int i0 = 0; i0 < parts; i0 += BATCH) {
+            if (i0 > 0) {
+                if (i0 % 32 == 0) weights(i0);
+                sums(i0);
+            }
+            if (i0 % 32 == 0) {
+#pragma unroll
+                for (int x = 0; x < AT_ONCE; ++x) { mi[x] = ex2_approx(mi[x] - m[x]); l[x] = fmaf(mi[x], li[x], l[x]); }      // now the factors
+            }
+#pragma unroll
+            for (int x = 0; x < AT_ONCE; ++x)
+#pragma unroll
+                for (int y = 0; y < BATCH; ++y) {
+                    const float w = __shfl_sync(0xffffffffu, mi[x], (i0 + y) & 31);
+                    if (i0 + y < parts)
+#pragma unroll
+                        for (int e = 0; e < VPL; ++e) o[x][e] = fmaf(v[x][y][e], w, o[x][e]);
+                }
+        }
+#pragma unroll
+        for (int x = 0; x < AT_ONCE; ++x) {
+#pragma unroll
+            for (int y = 16; y > 0; y >>= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], y);
+            if (r0 + x < rows) paged_finish<T, D>(p, c, c.t * TILE + r0 + x, lane * VPL, o[x], m[x], l[x]);
+        }
     }
 }
 
 template <typename T, int D, int THREADS, int TILE>
-__device__ __forceinline__ void paged_announce(const PagedParams& p, const PagedShares& sh, const PagedCursor (&split)[2], const int (&is_split)[2], int* flags, float* scratch) {
+__device__ __forceinline__ void paged_announce(const PagedParams& p, const PagedShares& sh, const PagedCursor (&split)[2], const int (&is_split)[2], int* flags) {
     __syncthreads();                                               // all sums are written, is_split and split are set
     if (!is_split[0] && !is_split[1]) return;
     if (threadIdx.x == 0) {
@@ -276,7 +292,7 @@ __device__ __forceinline__ void paged_announce(const PagedParams& p, const Paged
     }
     __syncthreads();
     for (int i = 0; i < 2; ++i)
-        if (flags[i]) paged_join<T, D, THREADS, TILE>(p, sh, split[i], scratch);
+        if (flags[i]) paged_join<T, D, THREADS, TILE>(p, sh, split[i]);
 }
 
 }  // namespace b200

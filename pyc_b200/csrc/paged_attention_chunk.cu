@@ -51,7 +51,6 @@ struct ChunkSmem {
     static constexpr int SPLIT_OFF = SHARES_OFF + sizeof(PagedShares);
     static constexpr int BYTES = SPLIT_OFF + 2 * sizeof(PagedCursor) + 16;
     static_assert(BYTES + 1024 <= 228 * 1024 && SHARES_OFF % 8 == 0, "shared memory of an SM");
-    static_assert(2 * 16 * (1 + 320) * 4 <= INFO_OFF, "the join's scratch: 16 rows of up to 320 parts");
 };
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -72,6 +71,13 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
 // 0x80 in each byte that is a NaN code.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
+// True in one lane of a converged warp; unlike a comparison of the lane number, it lets the compiler keep what the lane computes in
+// uniform registers, where tcgen05.mma takes its descriptors from.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
@@ -143,7 +149,7 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
         const int all_see = paged_limit(p, c.q, row0 / p.group);             // keys that every row sees
 
         if (warp == MMA_WARP) {
-            if (lane == 0) {
+            if (elect_one()) {
                 constexpr uint32_t HI = smem_desc_hi_sw128(1024);
                 const uint32_t q_lo0 = smem_desc_lo(sQ, 16), k_lo0 = smem_desc_lo(sK, 16), v_lo0 = smem_desc_lo(sV, KV_SLAB);
                 auto issue_qk = [&](int t, uint32_t b, uint32_t s) {         // S_t[s&1] = Q_t K_b^T
@@ -482,7 +488,7 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
     if (*reinterpret_cast<volatile int*>(p.status) != ST_OK) for (int i = 0; i < 2000; ++i) __nanosleep(1000);       // let what is in flight land
     tc_fence_after();
     if (warp == MMA_WARP) tmem_dealloc(tmem_base, TMEM_COLS);
-    paged_announce<T, D, THREADS, ROWS>(p, shares, split, is_split, flags, reinterpret_cast<float*>(smem));
+    paged_announce<T, D, THREADS, ROWS>(p, shares, split, is_split, flags);
 }
 
 template <typename T, int D>
