@@ -377,8 +377,8 @@ int pyc_b200_kv_write(const pyc_b200_kv_write_args* args, void* stream);
  * included.  Rows of out and lse from query_start[requests] on are not touched.  scale is positive and finite.
  * seq_lens beyond max_blocks * block_size count as that; scales outside 2^-40 .. 2^72 count as the nearer of the two.
  * q, out: bf16 or f16, rows q_stride / out_stride elements apart (0: contiguous; a multiple of 8; 16-byte aligned), heads
- * contiguous.  max_query is an upper bound of the queries of a request (a larger request's surplus rows are left undone),
- * and any number of rows may stand behind the last request.  workspace: pyc_b200_paged_attention_workspace_bytes(...) bytes,
+ * contiguous.  max_query is an upper bound of the queries of a request (a larger request's surplus rows are left undone;
+ * a tight one spares launches), and any number of rows may stand behind the last request.  workspace: pyc_b200_paged_attention_workspace_bytes(...) bytes,
  * 256-byte aligned, zeroed once before its first use; calls that may run at the same time need a workspace each (the
  * calls of one stream can share one, captured graphs that never overlap too). */
 typedef struct {
@@ -399,6 +399,7 @@ typedef struct {
     size_t q_stride, out_stride;
     float scale;
     int causal;
+    int rows;                      /* rows of q and out: no query beyond them is read or written; 0: query_start decides alone */
 } pyc_b200_paged_attention_args;
 size_t pyc_b200_paged_attention_workspace_bytes(int requests, int max_query, int heads, int kv_heads, int head_dim);
 int pyc_b200_paged_attention(const pyc_b200_paged_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);

@@ -105,7 +105,8 @@ class KvWriteArgs(C.Structure):
 class PagedAttentionArgs(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("dtype", "requests", "max_query", "heads", "kv_heads", "head_dim", "block_size", "num_blocks", "max_blocks")] + \
                [(n, C.c_void_p) for n in ("q", "k_cache", "v_cache", "k_scale", "v_scale", "block_table", "query_start", "seq_lens", "out", "lse")] + \
-               [("q_stride", C.c_size_t), ("out_stride", C.c_size_t), ("scale", C.c_float), ("causal", C.c_int)]
+               [("q_stride", C.c_size_t), ("out_stride", C.c_size_t), ("scale", C.c_float), ("causal", C.c_int),
+                ("rows", C.c_int)]
 
 
 class TokenLogprobsArgs(C.Structure):

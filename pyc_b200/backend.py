@@ -359,10 +359,10 @@ def paged_attention_workspace_bytes(requests, max_query, heads, kv_heads, head_d
 
 def paged_attention(dtype, requests, max_query, heads, kv_heads, head_dim, block_size, num_blocks, max_blocks, q, k_cache, v_cache, k_scale,
                     v_scale, block_table, query_start, seq_lens, out, scale, causal, workspace, workspace_bytes, lse=None, q_stride=0,
-                    out_stride=0, stream=0):
+                    out_stride=0, stream=0, rows=0):
     """Attention of a ragged batch of queries over the 8-bit paged cache."""
     a = abi.PagedAttentionArgs(dtype, requests, max_query, heads, kv_heads, head_dim, block_size, num_blocks, max_blocks, q, k_cache, v_cache,
-                               k_scale, v_scale, block_table, query_start, seq_lens, out, lse, q_stride, out_stride, scale, int(causal))
+                               k_scale, v_scale, block_table, query_start, seq_lens, out, lse, q_stride, out_stride, scale, int(causal), rows)
     _check(load().pyc_b200_paged_attention(C.byref(a), workspace, workspace_bytes, stream), "pyc_b200_paged_attention")
 
 

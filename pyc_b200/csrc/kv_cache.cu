@@ -25,7 +25,7 @@ constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_MAX_REQUESTS = 16384;    // two int arrays in shared memory: 128 KB
 
 __device__ __forceinline__ void plan_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // Exclusive block scan of a pair of 64-bit sums; `total` gets the sums over the block.

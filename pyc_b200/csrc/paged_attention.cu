@@ -538,6 +538,11 @@ int launch_short(const CUtensorMap& tmK, const CUtensorMap& tmV, const PagedPara
     return 0;
 }
 
+// Which kernel takes a request goes by its rows (queries times query heads of a key head).  Measured for 64 requests of 8000 keys,
+// 8 key heads, bf16, this file's kernel | the tcgen05 kernel: head_dim 128, 8 rows 181 | 423 us, 16 rows 229 (f16 279) | 423, 32 rows
+// 676 (spills) | 425; head_dim 64, 16 rows 169 | 384, 32 rows 292 | 385.
+constexpr int few_rows(int head_dim) { return head_dim == 128 ? 16 : 32; }
+
 constexpr size_t WS_COUNTERS = 4096;          // bytes: one int per CTA, at most 1024
 
 // Two slots of [rows][D + 2] floats per CTA, for the largest of the forms.
@@ -556,7 +561,7 @@ extern "C" {
 
 size_t pyc_b200_paged_attention_workspace_bytes(int requests, int max_query, int heads, int kv_heads, int head_dim) {
     if (requests < 1 || max_query < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
-    const bool many = static_cast<long long>(max_query) * (heads / kv_heads) > 32;
+    const bool many = static_cast<long long>(max_query) * (heads / kv_heads) > few_rows(head_dim);
     return WS_COUNTERS + (many ? std::max(partial_bytes(head_dim), paged_chunk_partial_bytes(head_dim)) : partial_bytes(head_dim));
 }
 
@@ -571,6 +576,7 @@ int pyc_b200_paged_attention(const pyc_b200_paged_attention_args* a, void* works
     if (a->requests < 1 || a->requests > 16384 || a->max_query < 1 || a->num_blocks < 1 || a->max_blocks < 1) {
         set_error("paged attention: requests (1 .. 16384), max_query, num_blocks and max_blocks must be positive"); return -1;
     }
+    if (a->rows < 0) { set_error("paged attention: %d rows", a->rows); return -1; }
     if (!(a->scale > 0.0f && a->scale < INFINITY)) { set_error("paged attention: scale must be positive and finite"); return -1; }
     if (a->kv_heads < 1 || a->heads < 1 || a->heads % a->kv_heads) { set_error("paged attention: %d heads over %d key heads", a->heads, a->kv_heads); return -1; }
     if (static_cast<long long>(a->num_blocks) * a->kv_heads > INT_MAX || static_cast<long long>(a->max_blocks) * a->block_size > INT_MAX ||
@@ -590,6 +596,7 @@ int pyc_b200_paged_attention(const pyc_b200_paged_attention_args* a, void* works
     p.q = a->q; p.out = a->out; p.lse = a->lse; p.k_scale = a->k_scale; p.v_scale = a->v_scale;
     p.table = a->block_table; p.starts = a->query_start; p.lens = a->seq_lens; p.q_stride = qs; p.out_stride = os;
     p.requests = a->requests; p.group = a->heads / a->kv_heads; p.kv_heads = a->kv_heads; p.max_query = a->max_query;
+    p.rows = a->rows > 0 ? a->rows : INT_MAX;
     p.max_blocks = a->max_blocks; p.num_blocks = a->num_blocks; p.block_size = a->block_size; p.shift = shift;
     p.scale_log2 = a->scale * 1.4426950408889634f; p.causal = a->causal != 0;
     p.counters = static_cast<int*>(workspace);
@@ -604,11 +611,11 @@ int pyc_b200_paged_attention(const pyc_b200_paged_attention_args* a, void* works
     const uint32_t box[3] = {128, static_cast<uint32_t>(GROUP / halves * a->head_dim / 128), 1};
     if (encode_tmap(&tmK, a->k_cache, 1, 3, dims, strides, box, true) != 0 || encode_tmap(&tmV, a->v_cache, 1, 3, dims, strides, box, true) != 0) return -1;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // Which kernel takes a request goes by its rows (queries times query heads of a key head), decided on the device: up to 8, 16
-    // or 32 rows (the smallest that covers max_query, or one token where that is beyond 32) the one for few rows, more than that the
-    // tcgen05 kernel.  MEASURED
+    // Decided on the device, by two launches where max_query allows both: up to 8, 16 or 32 rows (the smallest that covers max_query,
+    // or one token where max_query is beyond few_rows) the kernel for few rows, more than that the tcgen05 kernel.
     const long long most = static_cast<long long>(a->max_query) * p.group;
-    const int few = static_cast<int>(most <= 32 ? most : p.group <= 32 ? p.group : 0);
+    const int limit = few_rows(a->head_dim);
+    const int few = static_cast<int>(most <= limit ? most : p.group <= limit ? p.group : 0);
     p.cost = 2; p.unsplit = 8;               // an item's end takes about as long as two units' copies; a join takes 4 us, eight units 3
     const bool half = a->dtype == PYC_DTYPE_F16;
     const int upto = few <= 8 ? 8 : few <= 16 ? 16 : 32;
@@ -616,12 +623,12 @@ int pyc_b200_paged_attention(const pyc_b200_paged_attention_args* a, void* works
         p.rows_above = 0; p.rows_upto = upto;
         int rc;
 #define B200_SHORT(D, NQ) (half ? launch_short<__half, D, NQ>(tmK, tmV, p, halves, s) : launch_short<__nv_bfloat16, D, NQ>(tmK, tmV, p, halves, s))
-        if (a->head_dim == 128) rc = upto == 8 ? B200_SHORT(128, 1) : upto == 16 ? B200_SHORT(128, 2) : B200_SHORT(128, 4);
+        if (a->head_dim == 128) rc = upto == 8 ? B200_SHORT(128, 1) : B200_SHORT(128, 2);
         else rc = upto == 8 ? B200_SHORT(64, 1) : upto == 16 ? B200_SHORT(64, 2) : B200_SHORT(64, 4);
 #undef B200_SHORT
         if (rc != 0) return rc;
     }
-    if (most <= 32) return 0;
+    if (most <= limit) return 0;
     p.rows_above = few > 0 ? upto : 0; p.rows_upto = INT_MAX;
     return launch_paged_chunk(a->dtype, a->head_dim, p, a->k_cache, a->v_cache, s);
 }

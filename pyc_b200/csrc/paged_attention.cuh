@@ -15,6 +15,7 @@
 
 #include "kv_cache.cuh"
 #include "math.cuh"
+#include "ptx_sm100.cuh"
 
 namespace b200 {
 
@@ -29,6 +30,7 @@ struct PagedParams {
     const int* lens;
     size_t q_stride, out_stride;
     int requests, group, kv_heads, max_query, max_blocks, num_blocks, block_size, shift;
+    int rows;                       // of q and out
     int rows_above, rows_upto;      // this launch takes the requests with rows_above < queries * group <= rows_upto
     float scale_log2;               // softmax scale * log2(e)
     int causal;
@@ -44,7 +46,7 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedParams& p, int 
     PagedRequest q;
     q.start = __ldg(p.starts + r);
     q.full = max(0, __ldg(p.starts + r + 1) - q.start);
-    q.n = min(q.full, p.max_query);
+    q.n = q.start < 0 ? 0 : max(0, min(min(q.full, p.max_query), p.rows - q.start));
     q.len = static_cast<int>(min(static_cast<long long>(max(0, __ldg(p.lens + r))), static_cast<long long>(p.max_blocks) << p.shift));
     const long long rows = static_cast<long long>(q.n) * p.group;
     q.rows = rows > p.rows_above && rows <= p.rows_upto ? static_cast<int>(rows) : 0;
@@ -75,7 +77,8 @@ __device__ __forceinline__ long long paged_request_weight(const PagedParams& p, 
 struct PagedShares {
     long long lo, total, share;     // this CTA's first position; all weight; weight per CTA (one more for the first `extra` CTAs)
     int ctas, extra;                // CTAs that have a stretch (never more than weight, so none is empty)
-    int found_r, found_at;          // request of the first position, and its beginning relative to lo
+    int found_r;                    // request of the first position, and its beginning relative to lo
+    long long found_at;
     long long sums[32];
     int most[32];
 };
@@ -120,6 +123,10 @@ __device__ __forceinline__ bool paged_begin(const PagedParams& p, PagedCursor& c
     c.cost = p.cost;
     upto += before;
     if (total == 0) return false;
+    if (total > static_cast<long long>(gridDim.x) << 30) {         // positions within a stretch are ints: months of work, refused
+        if (threadIdx.x == 0) atomicCAS(p.status, ST_OK, ST_WAIT_TIMEOUT | (0x6f << 8));
+        return false;
+    }
     const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
     if (static_cast<int>(blockIdx.x) >= ctas) return false;
     const long long share = total / ctas;
@@ -135,19 +142,20 @@ __device__ __forceinline__ bool paged_begin(const PagedParams& p, PagedCursor& c
             at += n;
         }
         sh.lo = lo; sh.total = total; sh.share = share; sh.ctas = ctas; sh.extra = extra;
-        sh.found_r = r; sh.found_at = static_cast<int>(at - lo);
+        sh.found_r = r; sh.found_at = at - lo;
     }
     __syncthreads();
-    int at = sh.found_at;
+    long long at = sh.found_at;
     c.r = sh.found_r;
     c.q = paged_request(p, c.r);
     for (c.t = 0;; ++c.t) {
         c.units = paged_tile_units<TILE, UNIT>(p, c.q, c.t);
-        if (at + (c.units + p.cost) * p.kv_heads > 0) break;
-        at += (c.units + p.cost) * p.kv_heads;
+        const long long heads = static_cast<long long>(c.units + p.cost) * p.kv_heads;
+        if (at + heads > 0) break;
+        at += heads;
     }
-    c.h = -at / (c.units + p.cost);
-    c.item = at + c.h * (c.units + p.cost);
+    c.h = static_cast<int>(-at / (c.units + p.cost));
+    c.item = static_cast<int>(at + static_cast<long long>(c.h) * (c.units + p.cost));
     return c.to() > 0;
 }
 // To the CTA's next item; false, and the cursor as it was, when its stretch has no part of it.
@@ -207,7 +215,7 @@ __device__ __forceinline__ void paged_join(const PagedParams& p, const PagedShar
     // One warp per row; lane i has the maxima and weights of parts i, i + 32, .. and the values D / 32 i .. of the sums.  What is
     // asked for at once: the maxima and weights, and the sums of BATCH parts, of AT_ONCE rows (large tiles are split in two or
     // three, small ones in up to hundreds).
-    constexpr int VPL = D / 32, AT_ONCE = TILE >= 64 ? 4 : 1, BATCH = TILE >= 64 ? 4 : 16;
+    constexpr int VPL = D / 32, AT_ONCE = TILE >= 64 ? 4 : 1, BATCH = 4;
     const int lane = threadIdx.x & 31, rows = min(TILE, c.q.rows - c.t * TILE);
     for (int r0 = (threadIdx.x >> 5) * AT_ONCE; r0 < rows; r0 += THREADS / 32 * AT_ONCE) {
         float mi[AT_ONCE], li[AT_ONCE], m[AT_ONCE], l[AT_ONCE], o[AT_ONCE][VPL], v[AT_ONCE][BATCH][VPL];

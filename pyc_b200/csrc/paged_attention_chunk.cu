@@ -13,7 +13,7 @@
 //   warps 6-13   softmax, one query row per thread; they make the queries' operand first and write the result last
 // The roles meet at mbarriers only and walk the items each on its own, so that the next item's blocks come in and are converted
 // while the softmax warps write this one's result.  With one tile per CTA and two CTAs per SM, each with its own converters that
-// loaded the codes themselves, 2048-query chunks took 780 us instead of NEW us.
+// loaded the codes themselves, four chunks of 2048 queries over 7048 keys took 780 us instead of 415 us.
 //
 // Precision is that of paged_attention.cu: queries scaled per row by a power of two and then rounded to f16, which loses
 // what lies below 2^-24 of the row's largest; p' = 2^(score + log2 vs - m) as f16, the softmax's weight sum p' / vs in f32.
@@ -507,7 +507,7 @@ int paged_chunk_ctas() { return std::min(sm_count(), 320); }
 size_t paged_chunk_partial_bytes(int head_dim) { return static_cast<size_t>(paged_chunk_ctas()) * 2 * ROWS * (head_dim + 2) * sizeof(float); }
 
 int launch_paged_chunk(pyc_dtype dtype, int head_dim, PagedParams p, const void* k_cache, const void* v_cache, cudaStream_t s) {
-    // an item's queries, first blocks and result take about as long as ten units of 64 keys (0.5 us each with two CTAs on the SM)
+    // an item's queries, first blocks and result take about as long as ten units of 64 keys (1.7 us each)
     p.cost = 10; p.unsplit = 16;
     if (dtype == PYC_DTYPE_F16) return head_dim == 128 ? launch<__half, 128>(p, k_cache, v_cache, s) : launch<__half, 64>(p, k_cache, v_cache, s);
     return head_dim == 128 ? launch<__nv_bfloat16, 128>(p, k_cache, v_cache, s) : launch<__nv_bfloat16, 64>(p, k_cache, v_cache, s);

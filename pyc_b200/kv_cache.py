@@ -10,7 +10,11 @@
     cache.release(finished)                    # finished requests give their blocks back
 
 Everything that a step decides is decided on the device (lengths, tables, free list), nothing synchronises, and the arrays
-never move: plan .. advance can be captured as one CUDA graph and replayed after new_lens has been filled again.  The compute
+never move: plan .. advance can be captured as one CUDA graph and replayed after new_lens has been filled again.  Steps follow
+one another: all of a cache's calls go to one stream (or to streams that wait for one another), for they share its tables and
+its workspace, and between a plan and its advance the tables belong to that step.  max_query (the constructor's, or attend's
+for one call) bounds the new tokens of a request; rows of a request beyond it are left undone, and a tight bound spares
+launches.  The compute
 is the C-ABI library (include/pyc_b200.h); torch holds the buffers.  PyC has no cache and no ragged batch.
 """
 from . import abi, backend
@@ -36,6 +40,7 @@ class PagedKvCache:
         self.requests, self.num_blocks, self.block_size, self.max_blocks = requests, num_blocks, block_size, max_blocks
         self.max_tokens, self.max_query = max_tokens, min(max_query or max_tokens, max_tokens)
         self.heads, self.kv_heads, self.head_dim, self.layers = heads, kv_heads, head_dim, layers
+        self._planned = False                                       # between plan and advance
 
         def ints(*shape, fill=0, kind=torch.int32):
             return torch.full(shape, fill, dtype=kind, device=self.device)
@@ -71,11 +76,16 @@ class PagedKvCache:
             raise ValueError(f"{name}: shape {tuple(x.shape)} is not [tokens, {width // self.head_dim}, {self.head_dim}] or [tokens, {width}]")
         if not 1 <= x.shape[0] <= self.max_tokens:
             raise ValueError(f"{name}: {x.shape[0]} rows, max_tokens is {self.max_tokens}")
+        if x.shape[0] > 1 and (x.stride(0) < width or x.stride(0) % 8):
+            raise ValueError(f"{name}: rows {x.stride(0)} values apart, expected a multiple of 8 of at least {width}")
         return x.shape[0], (x.stride(0) if x.shape[0] > 1 else width)
 
     def plan(self, new_lens=None):
         """Tables and slots for a step that adds new_lens[r] tokens to request r (a device tensor, or a list; None: self.new_lens
-        as it is).  Check `status()` after it wherever the pool may run out; a step that could not be planned has no tokens."""
+        as it is).  Check `status()` after it wherever the pool may run out; a step that could not be planned has no tokens, and
+        after `status()` has raised for it another one may be planned."""
+        if self._planned:
+            raise RuntimeError("plan: the step before has not been advanced (its blocks would be lost)")
         if new_lens is not None:
             x = self.torch.as_tensor(new_lens, dtype=self.torch.int32)
             if tuple(x.shape) != (self.requests,):
@@ -85,11 +95,14 @@ class PagedKvCache:
                         self.new_lens.data_ptr(), self.free_blocks.data_ptr(), self.free_count.data_ptr(), self.block_table.data_ptr(),
                         self.query_start.data_ptr(), self.seq_lens.data_ptr(), self.slot_map.data_ptr(), self.positions.data_ptr(),
                         self.token_request.data_ptr(), self.result.data_ptr(), stream=self._stream())
+        self._planned = True
 
     def status(self):
         """(tokens, blocks taken) of the last plan; synchronises.  Raises when it could not be planned."""
         code, tokens, taken, missing = self.result.tolist()
         if code:
+            if code & 15:
+                self._planned = False                               # nothing was handed out
             what = ", ".join(text for bit, text in RESULT_ERRORS.items() if code & bit)
             raise backend.BackendError(f"kv plan: {what}" + (f" ({missing} missing)" if missing else ""))
         return tokens, taken
@@ -104,9 +117,12 @@ class PagedKvCache:
                          self.slot_map.data_ptr(), self.k_cache[layer].data_ptr(), self.v_cache[layer].data_ptr(),
                          self.k_scale[layer].data_ptr(), self.v_scale[layer].data_ptr(), k_stride=ks, v_stride=vs, stream=self._stream())
 
-    def attend(self, layer, q, out=None, lse=None, scale=None, causal=True):
+    def attend(self, layer, q, out=None, lse=None, scale=None, causal=True, max_query=None):
         """Attention of the step's queries over the cache.  Rows of `out` behind the last token are left as they were (zero when
-        it is made here).  `q` has at least as many rows as the step has tokens."""
+        it is made here); tokens of the step for which `q` has no row are left out."""
+        most = self.max_query if max_query is None else max_query
+        if not 1 <= most <= self.max_query:
+            raise ValueError(f"max_query {most} is not in 1 .. {self.max_query}")
         rows, qs = self._rows("q", q, self.heads * self.head_dim)
         if out is None:
             out = self.torch.zeros((rows, self.heads, self.head_dim), dtype=self.dtype, device=self.device)
@@ -116,21 +132,25 @@ class PagedKvCache:
         if lse is not None and (tuple(lse.shape) != (rows, self.heads) or lse.dtype != self.torch.float32 or not lse.is_contiguous() or
                                 lse.device != self.device):
             raise ValueError(f"lse must be contiguous float32 [{rows}, {self.heads}] on {self.device}")
-        backend.paged_attention(self._kind, self.requests, self.max_query, self.heads, self.kv_heads, self.head_dim, self.block_size,
+        backend.paged_attention(self._kind, self.requests, most, self.heads, self.kv_heads, self.head_dim, self.block_size,
                                 self.num_blocks, self.max_blocks, q.data_ptr(), self.k_cache[layer].data_ptr(),
                                 self.v_cache[layer].data_ptr(), self.k_scale[layer].data_ptr(), self.v_scale[layer].data_ptr(),
                                 self.block_table.data_ptr(), self.query_start.data_ptr(), self.seq_lens.data_ptr(), out.data_ptr(),
                                 scale if scale is not None else self.head_dim ** -0.5, causal, self.workspace.data_ptr(),
                                 self.workspace.numel(), lse=lse.data_ptr() if lse is not None else None, q_stride=qs, out_stride=os_,
-                                stream=self._stream())
+                                rows=rows, stream=self._stream())
         return out
 
     def advance(self):
         """The step's tokens become context of the next one."""
         self.context_lens.copy_(self.seq_lens)
+        self._planned = False
 
     def release(self, finished):
-        """Give back the blocks of the requests with finished[r] != 0 (a device tensor or a list); their length becomes 0."""
+        """Give back the blocks of the requests with finished[r] != 0 (a device tensor or a list); their length becomes 0.
+        Between steps only: after advance, before the next plan."""
+        if self._planned:
+            raise RuntimeError("release: the planned step has not been advanced")
         x = self.torch.as_tensor(finished).to(device=self.device, dtype=self.torch.int32).contiguous()
         if tuple(x.shape) != (self.requests,):
             raise ValueError(f"finished: shape {tuple(x.shape)}, expected ({self.requests},)")

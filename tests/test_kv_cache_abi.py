@@ -140,5 +140,39 @@ def test_cache_class_refuses_what_it_cannot_hold():
         c.status()
 
 
+def test_cache_class_refuses_overlapping_rows_and_steps_out_of_order(monkeypatch):
+    import torch
+    from pyc_b200.kv_cache import PagedKvCache
+    c = PagedKvCache(torch, requests=2, num_blocks=8, block_size=16, max_blocks=4, max_tokens=8, heads=4, kv_heads=2, head_dim=64, dtype=torch.bfloat16,
+                     device="cpu")
+    row = torch.zeros((1, 128), dtype=torch.bfloat16)
+    for bad in (row.expand(4, 128), torch.zeros(4 * 132, dtype=torch.bfloat16).as_strided((4, 128), (132, 1)), torch.zeros(600, dtype=torch.bfloat16).as_strided((4, 128), (64, 1))):
+        with pytest.raises(ValueError, match="values apart"):
+            c._rows("k", bad, 128)
+    with pytest.raises(ValueError, match="max_query"):
+        c.attend(0, torch.zeros((8, 256), dtype=torch.bfloat16), max_query=9)
+    monkeypatch.setattr(c, "_stream", lambda: 0)
+    monkeypatch.setattr(backend, "kv_plan", lambda *a, **k: None)
+    monkeypatch.setattr(backend, "kv_release", lambda *a, **k: None)
+    c.plan([1, 1])
+    with pytest.raises(RuntimeError):
+        c.plan([1, 1])
+    with pytest.raises(RuntimeError):
+        c.release([1, 0])
+    c.advance()
+    c.release([1, 0])
+    c.plan([1, 1])
+    c.result.copy_(torch.tensor([8, 0, 0, 1]))             # could not be planned: another one may be
+    with pytest.raises(backend.BackendError):
+        c.status()
+    c.plan([1, 0])
+
+
+def test_attention_refuses_a_negative_number_of_rows():
+    a = fill(abi.PagedAttentionArgs, **ATTEND, rows=-1)
+    assert backend.load().pyc_b200_paged_attention(C.byref(a), 0x10000, 1 << 30, None) == -1
+    assert "-1 rows" in backend.last_error()
+
+
 if __name__ == "__main__":
     sys.exit(pytest.main([__file__, "-q"]))
