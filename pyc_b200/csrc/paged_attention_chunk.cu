@@ -43,7 +43,8 @@ struct ChunkSmem {
     static constexpr int RAW = 4;                                        // stages of codes
     static constexpr int Q_BYTES = BQ * D * 2, KV_TILE = BK * D * 2, RAW_TILE = BK * D;
     static constexpr int K_OFF = TILES * Q_BYTES, V_OFF = K_OFF + 2 * KV_TILE, RAW_OFF = V_OFF + 2 * KV_TILE;
-    static constexpr int INFO_OFF = RAW_OFF + RAW * 2 * RAW_TILE;        // float4 [RING][4]: per block and 16 keys
+    static constexpr int OUT_OFF = RAW_OFF + RAW * 2 * RAW_TILE;         // per softmax warp 32 rows of 32 results, on their way out
+    static constexpr int INFO_OFF = OUT_OFF + 4 * TILES * 2048;          // float4 [RING][4]: per block and 16 keys
     static constexpr int NAN_OFF = INFO_OFF + RING * 64;                 // int [RING]: per item, whether a NaN value was left out
     static constexpr int BAR_OFF = NAN_OFF + RING * 4;
     static constexpr int NUM_BARS = 2 * RAW + 8 + 7 * TILES;             // raw full, empty | k full, empty, v full, empty (2 each) | per tile: q, s full (2), p full (2), pv done, o done
@@ -62,6 +63,8 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) { const __half2 h
 template <typename T> __device__ __forceinline__ float2 wide2(uint32_t w);
 template <> __device__ __forceinline__ float2 wide2<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 template <> __device__ __forceinline__ float2 wide2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <typename T> struct Bf16 { static constexpr bool value = false; };
+template <> struct Bf16<__nv_bfloat16> { static constexpr bool value = true; };
 template <typename T> __device__ __forceinline__ uint32_t narrow2(float a, float b);
 template <> __device__ __forceinline__ uint32_t narrow2<__nv_bfloat16>(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
 template <> __device__ __forceinline__ uint32_t narrow2<__half>(float a, float b) { return pack_f16(a, b); }
@@ -141,6 +144,54 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
     uint32_t pv = 0, done = 0;                           // blocks and items before this one of this softmax warp's tile (MMA warp: of tile 1, which has no
                                                          // part in items of up to 128 rows; tile 0 has one in all)
     bool ok = true;
+
+    // A softmax warp's tile and place in it, and what it knows of the row whose score it forms next.
+    const int t = (warp - SOFTMAX_WARP) >> 2, wq = warp & 3, in_tile = wq * 32 + lane;
+    const uint32_t lane_addr = tmem_base + t * TILE_COLS + (static_cast<uint32_t>(wq * 32) << 16);
+    float next_qs = 0.0f;                                // its scale
+    bool next_finite = true;                             // a row that is not becomes zeros, and NaN at the end if it sees a key
+    // The warp's 32 query rows of item x, each scaled to [1, 2) by a power of two, as f16 operand.  D / 8 lanes read one row.
+    auto queries = [&](const PagedCursor& x) {
+        const int row0 = x.t * ROWS, rows = min(ROWS, x.q.rows - row0);
+        if (t * BQ >= rows) return;
+        constexpr int LPR = D / 8, RPL = 32 / LPR, LOADS = 32 / RPL;
+        const int at_row = row0 + min(t * BQ + in_tile, rows - 1), token = at_row / p.group, head = x.h * p.group + (at_row - token * p.group);
+        const size_t row_at = (static_cast<size_t>(x.q.start) + token) * p.q_stride + static_cast<size_t>(head) * D;
+        uint4 u[LOADS];
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            u[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + __shfl_sync(0xffffffffu, row_at, i * RPL + lane / LPR)) + lane % LPR);
+        constexpr uint32_t INF = Bf16<T>::value ? 0x7f80 : 0x7c00;
+        uint32_t own = 0;                                // magnitude of the thread's own row
+        // at the ends of the range, where 2^e or 2^-e would be subnormal, to [0, 4)
+        auto exponent = [&](uint32_t bits) {
+            const float amax = wide2<T>(bits).x;
+            return amax > 0.0f && bits < INF ? min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -126), 126) : 0;
+        };
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+            uint32_t bits = 0, h[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) bits = __vmaxu2(bits, w[y] & 0x7fff7fffu);
+            bits = max(bits & 0xffffu, bits >> 16);
+#pragma unroll
+            for (int y = LPR / 2; y > 0; y >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, y));
+            const float down = exp2_int(-exponent(bits));
+            const uint32_t of_own = __shfl_sync(0xffffffffu, bits, (lane % RPL) * LPR);
+            if (lane / RPL == i) own = of_own;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) { const float2 f = wide2<T>(w[y]); h[y] = bits < INF ? pack_f16(f.x * down, f.y * down) : 0u; }
+            const int line = wq * 32 + i * RPL + lane / LPR, piece = lane % LPR;
+            sts128(sQ + t * SM::Q_BYTES + (piece >> 3) * Q_SLAB + line * 128 + (((piece & 7) ^ (line & 7)) << 4), h[0], h[1], h[2], h[3]);
+        }
+        next_qs = exp2_int(exponent(own)) * p.scale_log2;
+        next_finite = own < INF;
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full(t));
+    };
+    if (warp >= SOFTMAX_WARP) queries(c);
 
     for (uint32_t items = 0; ok; ++items) {
         const int j0 = c.from(), j1 = c.to(), blocks = j1 - j0;
@@ -257,95 +308,83 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                     sts128(line + (second << 4), odd ? h[0] : h[4], odd ? h[1] : h[5], odd ? h[2] : h[6], odd ? h[3] : h[7]);
                 }
             };
-            for (int j = j0; j < j1 && ok; ++j) {
-                const uint32_t b = n + (j - j0), st = b & 1, par = ((b >> 1) & 1) ^ 1, raw = sR + (b % RAW) * 2 * SM::RAW_TILE;
-                ok = __all_sync(0xffffffffu, mbar_wait(raw_full + 8 * (b % RAW), (b / RAW) & 1, p.status, 0x69));
-                if (!ok) break;
-                uint4 kx[LOADS], vx[LOADS];
+            // Tokens behind the last key and blocks outside the pool: whatever lies there becomes zero.
+            auto none = [&](int j, int i, const float4 (&in)[4]) {
+                const int x = (ct + i * CONVERTERS) / PER_ROW;
+                return j * BK + x >= kend || (x < 16 ? in[0].x : x < 32 ? in[1].x : x < 48 ? in[2].x : in[3].x) == 0.0f;
+            };
+            auto about = [&](uint32_t b, float4 (&in)[4]) {
 #pragma unroll
-                for (int i = 0; i < LOADS; ++i) { kx[i] = lds128(raw + (ct + i * CONVERTERS) * 16); vx[i] = lds128(raw + SM::RAW_TILE + (ct + i * CONVERTERS) * 16); }
+                for (int g = 0; g < 4; ++g) in[g] = info[(b % RING) * 4 + g];
+                return in[0].x == 0.0f || in[1].x == 0.0f || in[2].x == 0.0f || in[3].x == 0.0f;
+            };
+            auto keys = [&](int j) {
+                const uint32_t b = n + (j - j0), st = b & 1, raw = sR + (b % RAW) * 2 * SM::RAW_TILE;
+                if (!__all_sync(0xffffffffu, mbar_wait(raw_full + 8 * (b % RAW), (b / RAW) & 1, p.status, 0x69))) return false;
+                uint4 x[LOADS];
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) x[i] = lds128(raw + (ct + i * CONVERTERS) * 16);
+                float4 in[4];
+                if (about(b, in) || (j + 1) * BK > kend) {
+#pragma unroll
+                    for (int i = 0; i < LOADS; ++i) if (none(j, i, in)) x[i] = make_uint4(0, 0, 0, 0);
+                }
+                if (!__all_sync(0xffffffffu, mbar_wait(k_empty + 8 * st, ((b >> 1) & 1) ^ 1, p.status, 0x6a))) return false;
+                convert(sK + st * SM::KV_TILE, x);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(k_full + 8 * st);
+                return true;
+            };
+            auto values = [&](int j) {                                       // of a block whose keys this warp has converted
+                const uint32_t b = n + (j - j0), st = b & 1, raw = sR + (b % RAW) * 2 * SM::RAW_TILE;
+                uint4 x[LOADS];
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) x[i] = lds128(raw + SM::RAW_TILE + (ct + i * CONVERTERS) * 16);
                 const bool cut = (j + 1) * BK > all_see;
-                const float4 in[4] = {info[(b % RING) * 4], info[(b % RING) * 4 + 1], info[(b % RING) * 4 + 2], info[(b % RING) * 4 + 3]};
-                if (cut || in[0].x == 0.0f || in[1].x == 0.0f || in[2].x == 0.0f || in[3].x == 0.0f) {
-                    // tokens behind the last key and blocks outside the pool: whatever lies there becomes zero, and so do NaN values that some
-                    // row does not see (0 * NaN would reach it)
+                float4 in[4];
+                if (about(b, in) || cut) {
+                    // NaN values that some row does not see become zero too (0 * NaN would reach it)
                     bool nan = false;
 #pragma unroll
                     for (int i = 0; i < LOADS; ++i) {
-                        const int t = (ct + i * CONVERTERS) / PER_ROW;
-                        const bool none = j * BK + t >= kend || (t < 16 ? in[0].x : t < 32 ? in[1].x : t < 48 ? in[2].x : in[3].x) == 0.0f;
-                        uint32_t w[4] = {vx[i].x, vx[i].y, vx[i].z, vx[i].w};
+                        const bool zero = none(j, i, in);
+                        uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
                         for (int y = 0; y < 4; ++y) {
-                            if (none) w[y] = 0;
+                            if (zero) w[y] = 0;
                             const uint32_t z = cut ? nan_bytes(w[y]) : 0u;
                             nan |= z != 0;
                             w[y] &= ~((z >> 7) * 0xffu);
                         }
-                        vx[i] = make_uint4(w[0], w[1], w[2], w[3]);
-                        if (none) kx[i] = make_uint4(0, 0, 0, 0);
+                        x[i] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                     if (nan) left_out[items % RING] = 1;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(raw_empty + 8 * (b % RAW));
-                ok = __all_sync(0xffffffffu, mbar_wait(k_empty + 8 * st, par, p.status, 0x6a));
-                if (!ok) break;
-                convert(sK + st * SM::KV_TILE, kx);
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(k_full + 8 * st);
-                ok = __all_sync(0xffffffffu, mbar_wait(v_empty + 8 * st, par, p.status, 0x6b));
-                if (!ok) break;
-                convert(sV + st * SM::KV_TILE, vx);
+                if (!__all_sync(0xffffffffu, mbar_wait(v_empty + 8 * st, ((b >> 1) & 1) ^ 1, p.status, 0x6b))) return false;
+                convert(sV + st * SM::KV_TILE, x);
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(v_full + 8 * st);
+                return true;
+            };
+            // a block's keys before the values of the one before it: the products with them come first, and their buffer is free earlier
+            ok = keys(j0);
+            for (int j = j0; j < j1 && ok; ++j) {
+                if (j + 1 < j1) ok = keys(j + 1);
+                if (ok) ok = values(j);
             }
-        } else if ((warp - SOFTMAX_WARP) / 4 < tiles) {
-            const int t = (warp - SOFTMAX_WARP) / 4, wq = warp & 3, in_tile = wq * 32 + lane, row = t * BQ + in_tile;
-            const uint32_t lane_addr = tmem_base + t * TILE_COLS + (static_cast<uint32_t>(wq * 32) << 16);
-            const int at_row = row0 + min(row, rows - 1), token = at_row / p.group, head = c.h * p.group + (at_row - token * p.group);
+        } else {
+            const bool mine = t < tiles;
+            const int row = t * BQ + in_tile, at_row = row0 + min(row, rows - 1), token = at_row / p.group, head = c.h * p.group + (at_row - token * p.group);
             const int lim = paged_limit(p, c.q, token);
-            // ---- this thread's query row, scaled to [1, 2) by a power of two, as f16 operand.  The last products with the previous item's
-            // operand are over: their scores have been read.
-            float qs;
-            bool finite = true;                                              // a row that is not becomes zeros, and NaN at the end if it sees a key
-            {
-                const T* src = static_cast<const T*>(p.q) + (static_cast<size_t>(c.q.start) + token) * p.q_stride + static_cast<size_t>(head) * D;
-                float amax = 0.0f;
-                uint4 u[D / 8];
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        const float2 f = wide2<T>(w[y]);
-                        amax = max3(amax, fabsf(f.x), fabsf(f.y));
-                        finite &= fabsf(f.x) < INFINITY && fabsf(f.y) < INFINITY;
-                    }
-                }
-                // at the ends of the range, where 2^e or 2^-e would be subnormal, to [0, 4)
-                const int e = amax > 0.0f && finite ? min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -126), 126) : 0;
-                const float down = exp2_int(-e);
-                qs = exp2_int(e) * p.scale_log2;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-                    uint32_t h[4];
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) { const float2 f = wide2<T>(w[y]); h[y] = finite ? pack_f16(f.x * down, f.y * down) : 0u; }
-                    sts128(sQ + t * SM::Q_BYTES + (i >> 3) * Q_SLAB + in_tile * 128 + (((i & 7) ^ (in_tile & 7)) << 4), h[0], h[1], h[2], h[3]);
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q_full(t));
-            }
+            const float qs = next_qs;
+            const bool finite = next_finite;
             float m = -INFINITY, l = 0.0f;
             const int warp_sees = __shfl_sync(0xffffffffu, lim, 0);          // keys that every row of the warp sees
-            for (int i = 0; i < blocks && ok; ++i) {
+            for (int i = 0; i < blocks && mine && ok; ++i) {
                 const uint32_t b = n + i, s = pv + i, s_addr = lane_addr + (s & 1) * BK;
                 ok = __all_sync(0xffffffffu, mbar_wait(s_full(t, s & 1), (s >> 1) & 1, p.status, 0x6c));
                 if (!ok) break;
@@ -422,15 +461,27 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full(t, s & 1));
             }
-            // the last P V has a barrier of its own, one completion per item: this warp may come to it when any number have completed
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), done & 1, p.status, 0x6e));
+            // The next item's queries, before this one's result: its first products run meanwhile.  The last products with this tile's
+            // present operand are over, for their scores have been read.
             if (ok) {
+                PagedCursor next = c;
+                if (paged_next<ROWS, BK>(p, next)) queries(next);
+            }
+            // the last P V has a barrier of its own, one completion per item: this warp may come to it when any number have completed
+            if (mine && ok) ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), done & 1, p.status, 0x6e));
+            if (mine && ok) {
                 tc_fence_after();
                 const bool whole = j0 == 0 && j1 == c.units;
                 float* part = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + (j0 == 0 ? 1 : 0)) * (static_cast<size_t>(ROWS) * (D + 2));
                 const float ref = m == -INFINITY ? 0.0f : m;
                 if (!finite && l > 0.0f) l = __int_as_float(0x7fffffff);
-                T* out = static_cast<T*>(p.out) + (static_cast<size_t>(c.q.start) + token) * p.out_stride + static_cast<size_t>(head) * D;
+                // Results leave in 64 contiguous bytes per row: through 2 KB of shared memory, 16-byte pieces XORed with the row, a thread
+                // writes piece lane % 4 of rows lane / 4, lane / 4 + 8, ..
+                const size_t row_at = (static_cast<size_t>(c.q.start) + token) * p.out_stride + static_cast<size_t>(head) * D;
+                T* to[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) to[y] = static_cast<T*>(p.out) + __shfl_sync(0xffffffffu, row_at, y * 8 + (lane >> 2)) + (lane & 3) * 8;
+                const uint32_t pad = smem_u32(smem + SM::OUT_OFF) + (warp - SOFTMAX_WARP) * 2048;
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 // columns of NaN values that were left out and that this row sees
                 uint32_t nan_cols[D / 32];
@@ -453,21 +504,27 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                     uint32_t r[32];
                     tmem_ld_32x32(lane_addr + O_COL + x * 32, r);
                     tmem_ld_wait();
-                    if (row < rows) {
 #pragma unroll
-                        for (int y = 0; y < 32; y += 8) {
-                            float v[8];
+                    for (int y = 0; y < 32; y += 8) {
+                        float v[8];
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                v[e] = l == 0.0f ? 0.0f : __uint_as_float(r[y + e]);      // no key seen: whatever the products left
-                                if (nan_cols[x] >> (y + e) & 1u) v[e] = __int_as_float(0x7fffffff);
-                            }
-                            if (whole) *reinterpret_cast<uint4*>(out + x * 32 + y) = make_uint4(narrow2<T>(v[0] * inv, v[1] * inv), narrow2<T>(v[2] * inv, v[3] * inv), narrow2<T>(v[4] * inv, v[5] * inv), narrow2<T>(v[6] * inv, v[7] * inv));
-                            else {
-                                float* dst = part + row * D + x * 32 + y;
-                                __stcg(reinterpret_cast<float4*>(dst), make_float4(v[0], v[1], v[2], v[3]));
-                                __stcg(reinterpret_cast<float4*>(dst + 4), make_float4(v[4], v[5], v[6], v[7]));
-                            }
+                        for (int e = 0; e < 8; ++e) {
+                            v[e] = l == 0.0f ? 0.0f : __uint_as_float(r[y + e]);          // no key seen: whatever the products left
+                            if (nan_cols[x] >> (y + e) & 1u) v[e] = __int_as_float(0x7fffffff);
+                        }
+                        if (whole) sts128(pad + lane * 64 + (((y >> 3) ^ ((lane >> 1) & 3)) << 4), narrow2<T>(v[0] * inv, v[1] * inv), narrow2<T>(v[2] * inv, v[3] * inv), narrow2<T>(v[4] * inv, v[5] * inv), narrow2<T>(v[6] * inv, v[7] * inv));
+                        else if (row < rows) {
+                            float* dst = part + row * D + x * 32 + y;
+                            __stcg(reinterpret_cast<float4*>(dst), make_float4(v[0], v[1], v[2], v[3]));
+                            __stcg(reinterpret_cast<float4*>(dst + 4), make_float4(v[4], v[5], v[6], v[7]));
+                        }
+                    }
+                    __syncwarp();
+                    if (whole) {
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            const int rr = y * 8 + (lane >> 2);
+                            if (row - lane + rr < rows) *reinterpret_cast<uint4*>(to[y] + x * 32) = lds128(pad + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
                         }
                     }
                     __syncwarp();
@@ -477,7 +534,7 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                 tc_fence_before();
                 __syncwarp();
             }
-            pv += blocks; ++done;
+            if (mine) { pv += blocks; ++done; }
         }
         n += blocks;
         if (threadIdx.x == 0 && (j0 != 0 || j1 != c.units)) { split[j0 == 0 ? 1 : 0] = c; is_split[j0 == 0 ? 1 : 0] = 1; }
