@@ -215,7 +215,7 @@ __device__ __forceinline__ void paged_join(const PagedParams& p, const PagedShar
     // One warp per row; lane i has the maxima and weights of parts i, i + 32, .. and the values D / 32 i .. of the sums.  What is
     // asked for at once: the maxima and weights, and the sums of BATCH parts, of AT_ONCE rows (large tiles are split in two or
     // three, small ones in up to hundreds).
-    constexpr int VPL = D / 32, AT_ONCE = TILE >= 64 ? 4 : 1, BATCH = 4;
+    constexpr int VPL = D / 32, AT_ONCE = TILE >= 64 ? 2 : 1, BATCH = TILE >= 64 ? 2 : 4;
     const int lane = threadIdx.x & 31, rows = min(TILE, c.q.rows - c.t * TILE);
     for (int r0 = (threadIdx.x >> 5) * AT_ONCE; r0 < rows; r0 += THREADS / 32 * AT_ONCE) {
         float mi[AT_ONCE], li[AT_ONCE], m[AT_ONCE], l[AT_ONCE], o[AT_ONCE][VPL], v[AT_ONCE][BATCH][VPL];

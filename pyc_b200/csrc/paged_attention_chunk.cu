@@ -412,8 +412,7 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
             const uint32_t items = it.number, n = it.n;
             const int j0 = it.j0, j1 = it.j1, blocks = it.blocks, row0 = it.row0, rows = it.rows, all_see = it.all_see;
             const bool mine = t < it.tiles;
-            const int row = t * BQ + in_tile, at_row = row0 + min(row, rows - 1), token = at_row / p.group, head = c.h * p.group + (at_row - token * p.group);
-            const int lim = paged_limit(p, c.q, token);
+            const int row = t * BQ + in_tile, lim = paged_limit(p, c.q, (row0 + min(row, rows - 1)) / p.group);
             const float qs = next_qs;
             const bool finite = next_finite;
             float m = -INFINITY, l = 0.0f;
@@ -511,6 +510,7 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                 if (!finite && l > 0.0f) l = __int_as_float(0x7fffffff);
                 // Results leave in 64 contiguous bytes per row: through 2 KB of shared memory, 16-byte pieces XORed with the row, a thread
                 // writes piece lane % 4 of rows lane / 4, lane / 4 + 8, ..
+                const int at_row = row0 + min(row, rows - 1), token = at_row / p.group, head = c.h * p.group + (at_row - token * p.group);
                 const size_t row_at = (static_cast<size_t>(c.q.start) + token) * p.out_stride + static_cast<size_t>(head) * D;
                 T* to[4];
 #pragma unroll
