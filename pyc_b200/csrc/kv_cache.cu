@@ -21,6 +21,7 @@ namespace {
 // cluster repeats the scan over all requests in its own shared memory (8 bytes per request out of L2) and then fills its
 // share of the entries, finding the request of an entry by binary search in the scanned array.  The cluster barrier in the
 // middle lets the free count be updated in place: no CTA reads it after the barrier, CTA 0 writes it behind.
+// Measured: 8 requests of one token 3.6 us, 2000 requests with 43 K new tokens 14 us (1 MB of tables: latency and binary searches).
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_MAX_REQUESTS = 16384;    // two int arrays in shared memory: 128 KB
 
@@ -189,6 +190,8 @@ kv_release_kernel(int R, int bs, int block_shift, int num_blocks, int max_blocks
 // keys | values) takes the runs that begin in its group one after the other.  A thread holds eight 16-byte vectors, a CTA
 // block_size * head_dim / 2048 warps, so that a whole block's values of a head are loaded at once, kept in registers while
 // their largest magnitude is found, and written as codes: every value is read once.
+// Measured: 64 single tokens (8 heads of 128) 2.9 us; 13 K tokens of prompts (82 MB) 19 us = 4.3 TB/s; reading the values twice, once
+// for the magnitude, took 100 us.
 template <typename T> struct KvIn;
 template <> struct KvIn<__nv_bfloat16> {
     static constexpr uint32_t INF = 0x7f80;

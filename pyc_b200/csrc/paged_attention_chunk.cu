@@ -2,18 +2,26 @@
 // stretches, split items and their joining are those of paged_attention.cuh; an item has two tiles of 128 rows (queries times
 // query heads of a key head), a unit 64 keys.
 //
-// One CTA per SM, 14 warps:
-//   warp 0       TMEM owner and single-thread MMA issuer, for both tiles t in turn
+// One CTA per SM, 16 warps:
+//   warps 0, 1   one thread each issues the products of one tile t (warp 0 owns TMEM)
 //                  S_t[n&1] = Q_t K_n^T     128 x 64 x D    (tcgen05, f16, S in TMEM, two buffers per tile)
 //                  O_t     += P_n V_n       128 x D x 64    (P_n from TMEM, where S_n was; V as MN-major operand)
-//   warp 1       brings the blocks' codes in (bulk copies, RAW stages), with the scales of their 16-token groups
-//   warps 2-5    codes to f16 operands (exact, two codes per conversion) in the 128-byte-swizzled layout.  tcgen05 has no product of
+//   warp 2       brings the blocks' codes in (bulk copies, RAW stages), with the scales of their 16-token groups
+//   warp 3       idle: softmax warps have to begin at a multiple of four, for the TMEM lanes that they may read
+//   warps 4-7    codes to f16 operands (exact, two codes per conversion) in the 128-byte-swizzled layout.  tcgen05 has no product of
 //                e4m3 with 16-bit operands; splitting the queries into e4m3 terms, as the kernel for few rows does, would spare the
 //                keys' conversion but not the values', and 256 rows share each conversion here
-//   warps 6-13   softmax, one query row per thread; they make the queries' operand first and write the result last
-// The roles meet at mbarriers only and walk the items each on its own, so that the next item's blocks come in and are converted
-// while the softmax warps write this one's result.  With one tile per CTA and two CTAs per SM, each with its own converters that
-// loaded the codes themselves, four chunks of 2048 queries over 7048 keys took 780 us instead of 415 us.
+//   warps 8-15   softmax, one query row per thread; they make the next item's operand before they write an item's result
+// The roles meet at mbarriers only and walk the items each on its own, so that the next item's blocks come in, are converted and
+// multiplied while the softmax warps write this one's result.
+//
+// Measured: 4 requests with chunks of 2048 queries behind up to 5000 keys (8 x 4 heads of 128, bf16, 0.254 TFLOP) take 369 us = 690
+// TFLOP/s.  Of 2700 clocks per block of 64 keys and both tiles a softmax warp computes for 2200 (two warps share an XU whose
+// exponentials alone take 1024, and each goes load, maximum, exponentials, store in turn), the issuing threads wait for it 1300;
+// neither products (8 us), conversions (16 us) nor half of the exponentials (22 us) left out changed much.  Ways here: one tile per CTA, two
+// CTAs per SM, converters that load codes themselves 780 us; two tiles that share conversions 627; queries, results and operands in 16-byte
+// pieces without bank conflicts 601; descriptors in uniform registers (an elected lane) 415; an issuing warp per tile instead of one for
+// both 381; the join 369.
 //
 // Precision is that of paged_attention.cu: queries scaled per row by a power of two and then rounded to f16, which loses
 // what lies below 2^-24 of the row's largest; p' = 2^(score + log2 vs - m) as f16, the softmax's weight sum p' / vs in f32.
@@ -142,8 +150,7 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
     uint32_t pv = 0, done = 0;                           // blocks and items before this one of this warp's tile (tile 1 has no part in items of up to 128 rows)
     bool ok = true;
-    // Each role walks the items in a loop of its own.  (In one loop around the roles, what all need was spilled for the softmax warps'
-    // sake, and the MMA thread fetched it from local memory for every block: 407 us instead of 381 us with an issuing warp per tile.)
+    // Each role walks the items in a loop of its own.
     struct Item {
         uint32_t number, n;                              // items and blocks before this one: every role counts them alike
         int j0, j1, blocks, row0, rows, tiles, kend, all_see;

@@ -14,6 +14,8 @@
 // bisection over the ordered bits.  Many ties at tau (coarse logits, a vocabulary masked down to a few tokens) end in a scan of the
 // row from its start, which is where the ties that count are; see top_of_slice.
 //
+// Measured: 2048 x 131072 bf16 (537 MB) with 20 alternatives 119 us = 4.5 TB/s, bound by issue slots; 16 x 32768 f32 10.5 us.
+//
 // Rows are taken by one CTA each; where there are fewer rows than the SMs can hold, a cluster of 2, 4 or 8 CTAs shares a row
 // and its first CTA joins the others' statistics and candidates through distributed shared memory.
 //
@@ -498,7 +500,7 @@ token_logprobs_kernel(pyc_b200_token_logprobs_args p, int ctas) {
     }
 }
 
-// ---- gradient: reads and writes each element once, bound by that.  One CTA per row and chunk of GRAD_CHUNK vectors; 16-byte
+// ---- gradient: reads and writes each element once, bound by that: 2048 x 131072 bf16 (1.07 GB) 159 us = 6.8 TB/s, 61 x 50001 f32 4.5 us.  One CTA per row and chunk of GRAD_CHUNK vectors; 16-byte
 // accesses where logits and gradient lie equally to a 16-byte boundary, single elements otherwise.
 constexpr int GRAD_U = 4, GRAD_CHUNK = LT * GRAD_U * 2;
 
