@@ -379,7 +379,7 @@ int pyc_b200_kv_write(const pyc_b200_kv_write_args* args, void* stream);
  * q, out: bf16 or f16, rows q_stride / out_stride elements apart (0: contiguous; a multiple of 8; 16-byte aligned), heads
  * contiguous.  max_query is an upper bound of the queries of a request (a larger request's surplus rows are left undone;
  * a tight one spares launches), and any number of rows may stand behind the last request.  workspace: pyc_b200_paged_attention_workspace_bytes(...) bytes,
- * 256-byte aligned, zeroed once before its first use; calls that may run at the same time need a workspace each (the
+ * 256-byte aligned, zeroed once before its first use (and again after a call that ended with a device status); calls that may run at the same time need a workspace each (the
  * calls of one stream can share one, captured graphs that never overlap too). */
 typedef struct {
     pyc_dtype dtype;
