@@ -36,7 +36,7 @@ struct PagedParams {
     int causal;
     int cost, unsplit;              // weight of an item beside its units; items of up to so many units stay whole where the launch has none larger
     int* counters;                  // [CTAs], zero between calls
-    float* partials;                // [CTAs][2][tile rows * (head_dim + 2)]
+    float* partials;                // [CTAs][2][tile rows * (head_dim + 2)]: sums, maxima, weights
     int* status;
 };
 
@@ -187,8 +187,9 @@ __device__ __forceinline__ int paged_last(const PagedShares& s, const PagedCurso
 
 __device__ __forceinline__ float paged_clamp_scale(float s) { return fminf(fmaxf(s, 0x1p-40f), 0x1p72f); }
 
-__device__ __forceinline__ void paged_store2(__nv_bfloat16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
-__device__ __forceinline__ void paged_store2(__half* p, float a, float b) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b); }
+template <typename T> __device__ __forceinline__ uint32_t paged_pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t paged_pack2<__nv_bfloat16>(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+template <> __device__ __forceinline__ uint32_t paged_pack2<__half>(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
 
 // Result of row `row` of the item from its sums `o` (values d .. d + N - 1), weight `l` and reference maximum `m` (log2 units).
 template <typename T, int D, int N>
@@ -198,8 +199,15 @@ __device__ __forceinline__ void paged_finish(const PagedParams& p, const PagedCu
     const bool none = l == 0.0f;                                   // no key seen: zero and -inf
     const float inv = none ? 0.0f : 1.0f / l;
     T* dst = static_cast<T*>(p.out) + at * p.out_stride + static_cast<size_t>(head) * D + d;
+    uint32_t w[N / 2];
 #pragma unroll
-    for (int i = 0; i < N; i += 2) paged_store2(dst + i, none ? 0.0f : o[i] * inv, none ? 0.0f : o[i + 1] * inv);
+    for (int i = 0; i < N; i += 2) w[i / 2] = paged_pack2<T>(none ? 0.0f : o[i] * inv, none ? 0.0f : o[i + 1] * inv);
+    if constexpr (N == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (N == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = w[i / 2];
+    }
     if (p.lse && d == 0) p.lse[at * (static_cast<size_t>(p.group) * p.kv_heads) + head] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
@@ -212,70 +220,104 @@ __device__ __forceinline__ void paged_join(const PagedParams& p, const PagedShar
     const int first = paged_first(sh, c), parts = paged_last(sh, c) - first + 1;
     constexpr size_t SLOT = static_cast<size_t>(TILE) * (D + 2);
     auto slot = [&](int i) { return p.partials + (static_cast<size_t>(first + i) * 2 + (i == 0 ? 1 : 0)) * SLOT; };
-    // One warp per row; lane i has the maxima and weights of parts i, i + 32, .. and the values D / 32 i .. of the sums.  What is
-    // asked for at once: the maxima and weights, and the sums of BATCH parts, of AT_ONCE rows (large tiles are split in two or
-    // three, small ones in up to hundreds).  Rows x parts at once, large tiles: 4 x 4 396 us for the chunks of paged_attention_chunk.cu,
-    // 8 x 2 402, 4 x 2 370, 2 x 2 368, 1 x 2 388; small ones, 64 requests | one of 131 K keys: 1 x 16 107 | 61 us, 1 x 8 105 | 61, 1 x 4 104 | 60.
-    constexpr int VPL = D / 32, AT_ONCE = TILE >= 64 ? 2 : 1, BATCH = TILE >= 64 ? 2 : 4;
+    // One warp per row; lane i has the maxima and weights of parts i, i + 32, .. (there can be hundreds) and the values D / 32 i .. of
+    // the sums, of which it asks for BATCH parts at once: 16 took 107 us for 64 requests of 8000 keys | 61 us for one of 131 K,
+    // 8 105 | 61, 4 104 | 60.
+    constexpr int VPL = D / 32, BATCH = 4;
     const int lane = threadIdx.x & 31, rows = min(TILE, c.q.rows - c.t * TILE);
-    for (int r0 = (threadIdx.x >> 5) * AT_ONCE; r0 < rows; r0 += THREADS / 32 * AT_ONCE) {
-        float mi[AT_ONCE], li[AT_ONCE], m[AT_ONCE], l[AT_ONCE], o[AT_ONCE][VPL], v[AT_ONCE][BATCH][VPL];
+    for (int row = threadIdx.x >> 5; row < rows; row += THREADS / 32) {
+        float mi, li, o[VPL], v[BATCH][VPL];
         auto weights = [&](int i0) {         // of parts i0 + lane
-#pragma unroll
-            for (int x = 0; x < AT_ONCE; ++x) {
-                const float* ml = slot(min(i0 + lane, parts - 1)) + TILE * D + min(r0 + x, rows - 1);
-                mi[x] = __ldcg(ml); li[x] = __ldcg(ml + TILE);
-                if (i0 + lane >= parts) { mi[x] = -INFINITY; li[x] = 0.0f; }
-            }
+            const float* ml = slot(min(i0 + lane, parts - 1)) + TILE * D + row;
+            mi = __ldcg(ml); li = __ldcg(ml + TILE);
+            if (i0 + lane >= parts) { mi = -INFINITY; li = 0.0f; }
         };
         auto sums = [&](int i) {             // of parts i .. i + BATCH - 1 (beyond the last: the last's)
 #pragma unroll
-            for (int x = 0; x < AT_ONCE; ++x)
-#pragma unroll
-                for (int y = 0; y < BATCH; ++y) {
-                    const float* src = slot(min(i + y, parts - 1)) + min(r0 + x, rows - 1) * D + lane * VPL;
-                    if constexpr (VPL == 4) { const float4 u = __ldcg(reinterpret_cast<const float4*>(src)); v[x][y][0] = u.x; v[x][y][1] = u.y; v[x][y][2] = u.z; v[x][y][3] = u.w; }
-                    else { const float2 u = __ldcg(reinterpret_cast<const float2*>(src)); v[x][y][0] = u.x; v[x][y][1] = u.y; }
-                }
+            for (int y = 0; y < BATCH; ++y) {
+                const float* src = slot(min(i + y, parts - 1)) + row * D + lane * VPL;
+                if constexpr (VPL == 4) { const float4 u = __ldcg(reinterpret_cast<const float4*>(src)); v[y][0] = u.x; v[y][1] = u.y; v[y][2] = u.z; v[y][3] = u.w; }
+                else { const float2 u = __ldcg(reinterpret_cast<const float2*>(src)); v[y][0] = u.x; v[y][1] = u.y; }
+            }
         };
         weights(0);
         sums(0);
+        float m = mi, l = 0.0f;
+        for (int i = lane + 32; i < parts; i += 32) m = fmaxf(m, __ldcg(slot(i) + TILE * D + row));
 #pragma unroll
-        for (int x = 0; x < AT_ONCE; ++x) {
-            m[x] = mi[x]; l[x] = 0.0f;
-            for (int i = lane + 32; i < parts; i += 32) m[x] = fmaxf(m[x], __ldcg(slot(i) + TILE * D + min(r0 + x, rows - 1)));
+        for (int y = 16; y > 0; y >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, y));
+        if (m == -INFINITY) m = 0.0f;
 #pragma unroll
-            for (int y = 16; y > 0; y >>= 1) m[x] = fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], y));
-            if (m[x] == -INFINITY) m[x] = 0.0f;
-#pragma unroll
-            for (int y = 0; y < VPL; ++y) o[x][y] = 0.0f;
-        }
+        for (int y = 0; y < VPL; ++y) o[y] = 0.0f;
 #pragma unroll 1
         for (int i0 = 0; i0 < parts; i0 += BATCH) {
             if (i0 > 0) {
                 if (i0 % 32 == 0) weights(i0);
                 sums(i0);
             }
-            if (i0 % 32 == 0) {
+            if (i0 % 32 == 0) { mi = ex2_approx(mi - m); l = fmaf(mi, li, l); }      // now the factors
 #pragma unroll
-                for (int x = 0; x < AT_ONCE; ++x) { mi[x] = ex2_approx(mi[x] - m[x]); l[x] = fmaf(mi[x], li[x], l[x]); }      // now the factors
+            for (int y = 0; y < BATCH; ++y) {
+                const float w = __shfl_sync(0xffffffffu, mi, (i0 + y) & 31);
+                if (i0 + y < parts)
+#pragma unroll
+                    for (int e = 0; e < VPL; ++e) o[e] = fmaf(v[y][e], w, o[e]);
+            }
+        }
+#pragma unroll
+        for (int y = 16; y > 0; y >>= 1) l += __shfl_xor_sync(0xffffffffu, l, y);
+        paged_finish<T, D>(p, c, c.t * TILE + row, lane * VPL, o, m, l);
+    }
+}
+
+// The same for the large tiles of chunks, which are split in two or three: a thread has one row, and eight values of it at a time.  The
+// sums lie four values of all rows after four values of all rows, so that a warp stores and reads 512 bytes in a piece.
+template <typename T, int D, int THREADS, int TILE>
+__device__ __forceinline__ void paged_join_tile(const PagedParams& p, const PagedShares& sh, const PagedCursor& c) {
+    const int first = paged_first(sh, c), parts = paged_last(sh, c) - first + 1;
+    constexpr size_t SLOT = static_cast<size_t>(TILE) * (D + 2);
+    constexpr int STEP = THREADS / TILE, AT_ONCE = 4 * STEP <= D / 8 ? 4 : D / 8 / STEP;
+    static_assert(THREADS % TILE == 0 && D / 8 % (STEP * AT_ONCE) == 0, "whole rows");
+    const int in_tile = threadIdx.x % TILE, row = c.t * TILE + in_tile;
+    if (row >= c.q.rows) return;
+    auto slot = [&](int i) { return p.partials + (static_cast<size_t>(first + i) * 2 + (i == 0 ? 1 : 0)) * SLOT; };
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, __ldcg(slot(i) + TILE * D + in_tile));
+    if (m == -INFINITY) m = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) l = fmaf(ex2_approx(__ldcg(slot(i) + TILE * D + in_tile) - m), __ldcg(slot(i) + TILE * (D + 1) + in_tile), l);
+#pragma unroll 1
+    for (int g = threadIdx.x / TILE; g < D / 8; g += STEP * AT_ONCE) {
+        float o[AT_ONCE][8] = {};
+#pragma unroll 1
+        for (int i = 0; i < parts; i += 2) {
+            float w[2];
+            float4 v[2][AT_ONCE][2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const float* src = slot(min(i + y, parts - 1));
+                w[y] = __ldcg(src + TILE * D + in_tile);
+#pragma unroll
+                for (int x = 0; x < AT_ONCE; ++x)
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) v[y][x][z] = __ldcg(reinterpret_cast<const float4*>(src) + ((g + x * STEP) * 2 + z) * TILE + in_tile);
             }
 #pragma unroll
-            for (int x = 0; x < AT_ONCE; ++x)
+            for (int y = 0; y < 2; ++y) {
+                if (i + y >= parts) break;
+                const float f = ex2_approx(w[y] - m);
 #pragma unroll
-                for (int y = 0; y < BATCH; ++y) {
-                    const float w = __shfl_sync(0xffffffffu, mi[x], (i0 + y) & 31);
-                    if (i0 + y < parts)
+                for (int x = 0; x < AT_ONCE; ++x)
 #pragma unroll
-                        for (int e = 0; e < VPL; ++e) o[x][e] = fmaf(v[x][y][e], w, o[x][e]);
-                }
+                    for (int z = 0; z < 2; ++z) {
+                        o[x][z * 4] = fmaf(v[y][x][z].x, f, o[x][z * 4]); o[x][z * 4 + 1] = fmaf(v[y][x][z].y, f, o[x][z * 4 + 1]);
+                        o[x][z * 4 + 2] = fmaf(v[y][x][z].z, f, o[x][z * 4 + 2]); o[x][z * 4 + 3] = fmaf(v[y][x][z].w, f, o[x][z * 4 + 3]);
+                    }
+            }
         }
 #pragma unroll
-        for (int x = 0; x < AT_ONCE; ++x) {
-#pragma unroll
-            for (int y = 16; y > 0; y >>= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], y);
-            if (r0 + x < rows) paged_finish<T, D>(p, c, c.t * TILE + r0 + x, lane * VPL, o[x], m[x], l[x]);
-        }
+        for (int x = 0; x < AT_ONCE; ++x) paged_finish<T, D>(p, c, row, (g + x * STEP) * 8, o[x], m, l);
     }
 }
 
@@ -301,7 +343,10 @@ __device__ __forceinline__ void paged_announce(const PagedParams& p, const Paged
     }
     __syncthreads();
     for (int i = 0; i < 2; ++i)
-        if (flags[i]) paged_join<T, D, THREADS, TILE>(p, sh, split[i]);
+        if (flags[i]) {
+            if constexpr (TILE >= 64) paged_join_tile<T, D, THREADS, TILE>(p, sh, split[i]);
+            else paged_join<T, D, THREADS, TILE>(p, sh, split[i]);
+        }
 }
 
 }  // namespace b200

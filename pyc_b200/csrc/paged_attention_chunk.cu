@@ -73,9 +73,6 @@ template <> __device__ __forceinline__ float2 wide2<__nv_bfloat16>(uint32_t w) {
 template <> __device__ __forceinline__ float2 wide2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 template <typename T> struct Bf16 { static constexpr bool value = false; };
 template <> struct Bf16<__nv_bfloat16> { static constexpr bool value = true; };
-template <typename T> __device__ __forceinline__ uint32_t narrow2(float a, float b);
-template <> __device__ __forceinline__ uint32_t narrow2<__nv_bfloat16>(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
-template <> __device__ __forceinline__ uint32_t narrow2<__half>(float a, float b) { return pack_f16(a, b); }
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
@@ -553,11 +550,11 @@ paged_chunk_kernel(const __grid_constant__ PagedParams p, const uint8_t* __restr
                             v[e] = l == 0.0f ? 0.0f : __uint_as_float(r[y + e]);          // no key seen: whatever the products left
                             if (nan_cols[x] >> (y + e) & 1u) v[e] = __int_as_float(0x7fffffff);
                         }
-                        if (whole) sts128(pad + lane * 64 + (((y >> 3) ^ ((lane >> 1) & 3)) << 4), narrow2<T>(v[0] * inv, v[1] * inv), narrow2<T>(v[2] * inv, v[3] * inv), narrow2<T>(v[4] * inv, v[5] * inv), narrow2<T>(v[6] * inv, v[7] * inv));
+                        if (whole) sts128(pad + lane * 64 + (((y >> 3) ^ ((lane >> 1) & 3)) << 4), paged_pack2<T>(v[0] * inv, v[1] * inv), paged_pack2<T>(v[2] * inv, v[3] * inv), paged_pack2<T>(v[4] * inv, v[5] * inv), paged_pack2<T>(v[6] * inv, v[7] * inv));
                         else if (row < rows) {
-                            float* dst = part + row * D + x * 32 + y;
-                            __stcg(reinterpret_cast<float4*>(dst), make_float4(v[0], v[1], v[2], v[3]));
-                            __stcg(reinterpret_cast<float4*>(dst + 4), make_float4(v[4], v[5], v[6], v[7]));
+                            float4* dst = reinterpret_cast<float4*>(part) + (x * 8 + y / 4) * ROWS + row;
+                            __stcg(dst, make_float4(v[0], v[1], v[2], v[3]));
+                            __stcg(dst + ROWS, make_float4(v[4], v[5], v[6], v[7]));
                         }
                     }
                     __syncwarp();
