@@ -1,4 +1,4 @@
-// Attention over the 8-bit paged cache for many query rows per key head: chunks of prompts, bound by the products.  Items,
+// Attention over the 8-bit paged cache for many query rows per key head: chunks of prompts, bound by products and softmax.  Items,
 // stretches, split items and their joining are those of paged_attention.cuh; an item has two tiles of 128 rows (queries times
 // query heads of a key head), a unit 64 keys.
 //
@@ -15,13 +15,14 @@
 // The roles meet at mbarriers only and walk the items each on its own, so that the next item's blocks come in, are converted and
 // multiplied while the softmax warps write this one's result.
 //
-// Measured: 4 requests with chunks of 2048 queries behind up to 5000 keys (8 x 4 heads of 128, bf16, 0.254 TFLOP) take 369 us = 690
-// TFLOP/s.  Of 2700 clocks per block of 64 keys and both tiles a softmax warp computes for 2200 (two warps share an XU whose
+// Measured: 4 requests with chunks of 2048 queries behind up to 5000 keys (8 x 4 heads of 128, bf16, 0.254 TFLOP) take 347 us = 732
+// TFLOP/s; 8 prompts of 1000 tokens with nothing before them 177 us, of which 7 items per CTA take about 5 us each at their ends.
+// Of 2700 clocks per block of 64 keys and both tiles a softmax warp computes for 2200 (two warps share an XU whose
 // exponentials alone take 1024, and each goes load, maximum, exponentials, store in turn), the issuing threads wait for it 1300;
 // neither products (8 us), conversions (16 us) nor half of the exponentials (22 us) left out changed much.  Ways here: one tile per CTA, two
 // CTAs per SM, converters that load codes themselves 780 us; two tiles that share conversions 627; queries, results and operands in 16-byte
 // pieces without bank conflicts 601; descriptors in uniform registers (an elected lane) 415; an issuing warp per tile instead of one for
-// both 381; the join 369.
+// both 381; the join, a row per thread and sums in 512-byte pieces, 347.
 //
 // Precision is that of paged_attention.cu: queries scaled per row by a power of two and then rounded to f16, which loses
 // what lies below 2^-24 of the row's largest; p' = 2^(score + log2 vs - m) as f16, the softmax's weight sum p' / vs in f32.
@@ -599,7 +600,8 @@ int paged_chunk_ctas() { return std::min(sm_count(), 320); }
 size_t paged_chunk_partial_bytes(int head_dim) { return static_cast<size_t>(paged_chunk_ctas()) * 2 * ROWS * (head_dim + 2) * sizeof(float); }
 
 int launch_paged_chunk(pyc_dtype dtype, int head_dim, PagedParams p, const void* k_cache, const void* v_cache, cudaStream_t s) {
-    // an item's queries, first blocks and result take about as long as ten units of 64 keys (1.7 us each)
+    // an item's queries, first blocks and result weigh as much as this many units of 64 keys: 3 373 us, 6 357, 10 346, 14 348, 20 357 for
+    // 2048-query chunks; 8 prompts of 1000 tokens 223, 192, 176, 183, 183
     p.cost = 10; p.unsplit = 16;
     if (dtype == PYC_DTYPE_F16) return head_dim == 128 ? launch<__half, 128>(p, k_cache, v_cache, s) : launch<__half, 64>(p, k_cache, v_cache, s);
     return head_dim == 128 ? launch<__nv_bfloat16, 128>(p, k_cache, v_cache, s) : launch<__nv_bfloat16, 64>(p, k_cache, v_cache, s);
