@@ -457,6 +457,16 @@ def test_many_short_requests(backend):
     b.check(*b.run(backend))
 
 
+@pytest.mark.parametrize("dtype, D, G, bs", [(BF16, 64, 8, 16), (F16, 128, 8, 32), (BF16, 128, 16, 128)])
+def test_many_chunks_of_one_and_two_tiles(backend, dtype, D, G, bs):
+    """More items than CTAs: each walks several, of 33 to 320 rows in any order, with requests of few rows and of none between."""
+    rng = np.random.default_rng(D + G)
+    new = [int(x) for x in rng.choice([0, 1, 2, 5, 9, 16, 17, 20], 260)]
+    context = [int(x) for x in rng.choice([0, 1, 30, 70, 200], 260)]
+    b = Batch(context, new, 2, G, D, bs, dtype, seed=G)
+    b.check(*b.run(backend))
+
+
 def test_a_request_longer_than_its_table_row_counts_as_that_long(backend):
     b = Batch([60], [4], 2, 2, 64, 16, BF16, seed=16)
     b.lens[0] = 1 << 30

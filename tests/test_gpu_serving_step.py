@@ -207,3 +207,29 @@ def test_two_attentions_at_once_with_a_workspace_each(backend, new):
         for o in some:
             assert torch.equal(o, a)
     assert backend.device_status() == 0
+
+
+def test_two_graphs_share_a_workspace(backend):
+    """A captured step of single tokens and one of chunks on the same cache, replayed in turn, give what eager calls give."""
+    import torch
+    s = Server(backend, torch.float16, 3, 64, 16, 20, 300, 4, 2, 128, 150, seed=9)
+    for new in ([140, 90, 60], [1, 1, 1]):
+        s.feed(new)
+        s.device_step()
+    q = s.qkv[1][:3, :8 * 128].contiguous()
+    eager, eager_all = s.c.attend(1, q, max_query=1), s.c.attend(1, q)
+    torch.cuda.synchronize()
+    assert torch.equal(eager, eager_all)                              # with and without room for chunks
+    graphs, outs = [], [torch.zeros_like(eager) for _ in range(2)]
+    for out, most in zip(outs, (1, None)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            s.c.attend(1, q, out=out, max_query=most)
+        graphs.append(g)
+    for _ in range(5):
+        for g, out in zip(graphs, outs):
+            out.zero_()
+            g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], eager) and torch.equal(outs[1], eager)
+    assert backend.device_status() == 0
